@@ -48,6 +48,7 @@ extern "C" {
                            ztq calls are safe; a caller whose own kernel writes weights and triggers its dependents
                            early (griddepcontrol.launch_dependents) directly in front of a ztq launch passes this flag. */
 #define ZTQ_PLAIN  32   /* force the plain (non-streaming) kernel              */
+#define ZTQ_ROPE_PAIRS 128 /* rotary positions turn interleaved pairs (2i, 2i+1) instead of halves (i, i + rot_dim/2) */
 #define ZTQ_FP32_DECODE 64 /* decode codes to fp32 in registers instead of the exact integer block dot */
 
 /* ---- drop-in replacements: same names, arguments and meaning as the
@@ -290,6 +291,114 @@ cudaError_t ztq_dequantize(int fmt, const void* w, const void* meta_or_null, flo
  * N % 4 columns (multiply, then add), which is the order of that routine.  x: fp16, or float32 with ZTQ_X_F32.
  * A correctness path for that operand layout, not a tuned kernel.  Flags: ZTQ_X_F32, ZTQ_NO_PDL. */
 cudaError_t ztq_matmul_wkn_f32(const void* x, const float* w_kn, float* y, int M, int K, int N, int flags, cudaStream_t stream);
+
+/* ==== the decode step around the projections ================================
+ * What stands between two quantized projections of a decode step: the plan of the step (block tables, slots), rotary
+ * positions with the append of keys and values to a paged 8-bit cache, attention over that cache, and the token drawn
+ * from the logits.  No counterpart on the reference's quantized path (its rope, paged attention and argmax kernels,
+ * internal/cuda/kernels/, work on float32 caches with host-built tables).  All pointers belong to the current device.
+ * All of these are safe to capture; lengths, tables and slots are read on the device, so one captured graph serves steps
+ * of any lengths within the sizes given on the host. */
+
+/* The plan of a step.  Per sequence b: ctx_len[b] tokens are cached, new_len[b] >= 0 tokens come in this step, or
+ * new_len[b] == -1 ends the sequence and gives its blocks back.
+ *   block_table [sequences][table_width]  blocks of a sequence in order; the entries this step needs are filled in, all
+ *                                         others are left as they were
+ *   ring [pool_blocks], ring_state {head, count}   free blocks: `count` of them from `head` on, wrapping around.  New
+ *                                         blocks are taken from the head in the order of the sequences; blocks given
+ *                                         back go behind the last one and are used from the next step on.
+ *   ring_state_out {head, count}          may be ring_state itself
+ *   query_start [sequences + 1]           first row of each sequence among the step's rows, then the number of rows
+ *   positions, slots [max_tokens]         per row: position, and block * block_size + offset in the cache; rows behind
+ *                                         the last sequence get position 0 and slot -1 (the append skips them)
+ *   kv_len [sequences]                    tokens in the cache after the append (0: not in this step)
+ *   next_len [sequences]                  ctx_len of the next step (may be ctx_len itself)
+ *   status [sequences]                    0, or why a sequence gets nothing in this step (slots -1, kv_len 0, next_len =
+ *                                         ctx_len): 1 not enough free blocks, 2 table_width too small, 3 max_tokens
+ *                                         too small, 4 a negative or impossible length
+ * When blocks run short, a sequence is refused if its blocks and those of all sequences before it that ask for any
+ * exceed the free ones.  block_size: 16, 32, 64 or 128; sequences <= 4096.  Flags: ZTQ_NO_PDL. */
+cudaError_t ztq_kv_plan(const int* ctx_len, const int* new_len, int* block_table, int* ring, const int* ring_state, int* ring_state_out,
+                        int* next_len, int* kv_len, int* query_start, int* positions, int* slots, int* status, int sequences, int table_width,
+                        int block_size, int pool_blocks, int max_tokens, int flags, cudaStream_t stream);
+
+/* Rotary positions.  table [rows][rot_dim / 2] of float32 {cos, sin} of position * frequency, times `magnitude` (0: 1);
+ * made once per model by ztq_rope_table (angles in 64 bits) for positions first .. first + rows - 1.
+ * frequency i = base^(-2i / rot_dim), then
+ *   ZTQ_ROPE_LINEAR    divided by factor
+ *   ZTQ_ROPE_BY_TURNS  kept where it makes turns_high turns or more over original_positions, divided by factor where it
+ *                      makes turns_low or fewer, a linear blend in the number of turns between
+ *   ZTQ_ROPE_BY_DIM    the same, the blend linear in the dimension between those of turns_high (rounded down) and
+ *                      turns_low (rounded up)
+ * rot_dim: a multiple of 16 up to 256 and the head; what lies behind it in a head passes unchanged. */
+#define ZTQ_ROPE_UNSCALED 0
+#define ZTQ_ROPE_LINEAR   1
+#define ZTQ_ROPE_BY_TURNS 2
+#define ZTQ_ROPE_BY_DIM   3
+typedef struct ZtqRopeSpec {
+    double base, factor, turns_low, turns_high, original_positions, magnitude;
+    int rot_dim, scaling;
+} ZtqRopeSpec;
+cudaError_t ztq_rope_table(void* table, int first, int rows, const ZtqRopeSpec* spec, int flags, cudaStream_t stream);
+/* y[t, h] = x[t, h] rotated to positions[t]; strides in elements, head_dim contiguous and a multiple of 16 up to 256.
+ * y may be x (same strides and type).  A position outside the table makes the rotated part of its row NaN and sets the
+ * device error word to 6.  Flags: ZTQ_X_F32, ZTQ_Y_F32, ZTQ_ROPE_PAIRS, ZTQ_NO_PDL. */
+cudaError_t ztq_rope(const void* x, void* y, int tokens, int heads, int head_dim, long long x_token, long long x_head, long long y_token,
+                     long long y_head, const void* table, int table_rows, int rot_dim, const int* positions, int flags, cudaStream_t stream);
+
+/* One layer's paged cache: int8 codes, a value is its code times the scale of its (block, head).  Element d of token o of
+ * head h of block b stands at b * block_stride + (h * block_size + o) * head_dim + d of k and of v (block_stride in bytes, a
+ * multiple of 16, so blocks of several layers, or of k and v, may interleave); scales are [blocks][kv_heads].
+ * block_size 16, 32, 64 or 128; head_dim a multiple of 16 up to 256 (attention: 64, 128 or 256); k, v 16-byte aligned. */
+typedef struct ZtqKvCache {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    long long block_stride;
+    int blocks, kv_heads, block_size, head_dim;
+} ZtqKvCache;
+
+/* Rotates the queries into q_out (q_heads 0: none; q_out may be q) and appends the step's keys (rotated) and values to the
+ * cache at `slots` (negative: the row is skipped).  table NULL: nothing is rotated.  Strides in elements.
+ * The scale of a (block, head) becomes the smallest power of two that holds the new rows' largest value in 127 steps, or
+ * stays if it is larger already and the block held rows of the sequence (slot offset > 0); codes in the block are rounded
+ * to a grown scale.  A block whose new rows are not finite gets the scale NaN until it is begun anew.
+ * The rows of one block stand one after the other with consecutive slots, as ztq_kv_plan lays them out, and no slot comes
+ * twice; a row out of order behind one of its block, or a slot behind the cache, is skipped and sets the device error
+ * word to 5.  Flags: ZTQ_X_F32 (q, k, v), ZTQ_Y_F32 (q_out), ZTQ_ROPE_PAIRS, ZTQ_NO_PDL. */
+cudaError_t ztq_rope_append_q8(const void* q, const void* k, const void* v, void* q_out, long long q_token, long long q_head, long long k_token,
+                               long long k_head, long long v_token, long long v_head, long long qo_token, long long qo_head, int tokens, int q_heads,
+                               const void* table, int table_rows, int rot_dim, const int* positions, const int* slots, const ZtqKvCache* cache,
+                               int flags, cudaStream_t stream);
+/* The cache's dequantizer: k_out, v_out [tokens][kv_heads][head_dim] (either may be NULL; fp16, or float32 with ZTQ_Y_F32)
+ * = the cache's rows at `slots`; a slot outside the cache leaves its row as it was. */
+cudaError_t ztq_kv_read_q8(const ZtqKvCache* cache, const int* slots, int tokens, void* k_out, void* v_out, int flags, cudaStream_t stream);
+
+/* y[t, h] = attention of query row t, head h over its sequence's cached tokens: causal (the last row of a sequence stands
+ * at position kv_len - 1), and with window > 0 only over the last `window` positions up to its own.  q_heads is a multiple
+ * of kv_heads; head h reads kv head h / (q_heads / kv_heads).  Rows of sequence b: query_start[b] .. query_start[b + 1];
+ * rows behind the last sequence are left as they were; a row that sees nothing becomes 0.  scale_bits: the softmax
+ * scale's float32 bits.  max_new: most rows of one sequence (a sequence with more is left out and sets the device error
+ * word to 8).  A block table entry outside the cache hides its tokens and sets the error word to 7.
+ * workspace: >= ztq_attn_q8_workspace_bytes(...) of the same sizes, 16-byte aligned, overwritten; calls that share one must not overlap on the GPU
+ * (two captured graphs that may run at once need one each).  sequences <= 4096.
+ * With ZTQ_X_F32 or ZTQ_Y_F32 both products are done to fp32 accuracy.  Flags: ZTQ_X_F32, ZTQ_Y_F32, ZTQ_NO_PDL. */
+size_t ztq_attn_q8_workspace_bytes(int tokens, int sequences, int max_new, int q_heads, int kv_heads, int head_dim);
+cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_head, long long y_token, long long y_head, int tokens, int q_heads,
+                        const int* query_start, const int* kv_len, const int* block_table, int sequences, int table_width, int max_new, int window,
+                        unsigned scale_bits, const ZtqKvCache* cache, void* workspace, size_t workspace_bytes, int flags, cudaStream_t stream);
+
+/* One token per row of logits [rows][vocab] (row_stride in elements; fp16, or float32 with ZTQ_X_F32) from uniform[row] in
+ * [0, 1).  Tokens in order of (logit descending, index ascending), w = exp((logit - largest) / temperature); the first
+ * top_k stay (<= 0: all), of those the shortest prefix with top_p of their mass (at least one token; >= 1: all), of those
+ * the ones with w >= min_p; the token is the first by index whose running sum of w exceeds uniform times the sum.
+ * temperature 0 takes the first of the order.  Per-row arrays; temperature, top_k, top_p, min_p may be NULL (1, all,
+ * all, all).  logprob (may be NULL): log of the token's share of what was kept.  -inf and NaN are never drawn; a row
+ * with nothing else gives token -1 and logprob NaN.  vocab <= ZTQ_SAMPLE_MAX_VOCAB.  Flags: ZTQ_X_F32, ZTQ_NO_PDL. */
+#define ZTQ_SAMPLE_MAX_VOCAB 389120
+cudaError_t ztq_sample(const void* logits, long long row_stride, int rows, int vocab, const float* temperature, const int* top_k,
+                       const float* top_p, const float* min_p, const float* uniform, int* token, float* logprob, int flags, cudaStream_t stream);
 
 /* ---- probes ---------------------------------------------------------------- */
 /* The launch plan the first launch of a call with these arguments gets on a device of `sms` SMs (host

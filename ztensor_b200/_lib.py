@@ -58,6 +58,14 @@ SIGNATURES = {
     "ztq_quantize_w4g": [_vp, _vp, _vp, _ll, _i, _i, _vp],
     "ztq_dequantize": [_i, _vp, _vp, _vp, _ll, _i, _vp],
     "ztq_matmul_wkn_f32": [_vp, _vp, _vp, _i, _i, _i, _i, _vp],
+    "ztq_kv_plan": [_vp] * 12 + [_i] * 6 + [_vp],
+    "ztq_rope_table": [_vp, _i, _i, _vp, _i, _vp],
+    "ztq_rope": [_vp, _vp, _i, _i, _i, _ll, _ll, _ll, _ll, _vp, _i, _i, _vp, _i, _vp],
+    "ztq_rope_append_q8": [_vp] * 4 + [_ll] * 8 + [_i, _i, _vp, _i, _i, _vp, _vp, _vp, _i, _vp],
+    "ztq_kv_read_q8": [_vp, _vp, _i, _vp, _vp, _i, _vp],
+    "ztq_attn_q8_workspace_bytes": [_i] * 6,
+    "ztq_attn_q8": [_vp, _vp, _ll, _ll, _ll, _ll, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, C.c_uint, _vp, _vp, C.c_size_t, _i, _vp],
+    "ztq_sample": [_vp, _ll, _i, _i] + [_vp] * 7 + [_i, _vp],
     "ztq_describe_plan": [_i, _i, _i, _i, _i, _i, C.POINTER(C.c_int)],
     "ztq_probe_launch": [_i, _i, _i, _i, _vp],
     "ztq_check_sm100": [],

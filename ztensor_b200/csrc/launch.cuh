@@ -1,0 +1,75 @@
+// launch.cuh -- host helpers shared by the translation units of libztq_sm100a.so.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+
+#include <atomic>
+
+namespace ztq {
+
+static inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+struct DeviceInfo {
+    int sms = 0;
+    int major = 0;
+};
+
+static DeviceInfo device_info() {
+    // Queried per call: cheap attribute reads, no cached mutable state.
+    DeviceInfo d;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return d;
+    cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
+    cudaDeviceGetAttribute(&d.major, cudaDevAttrComputeCapabilityMajor, dev);
+    return d;
+}
+
+template <typename Kern, typename... Args>
+static cudaError_t launch(Kern kern, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// The same for a grid of clusters of `cluster` CTAs along x.
+template <typename Kern, typename... Args>
+static cudaError_t launch_cluster(Kern kern, dim3 grid, int cluster, dim3 block, size_t smem, cudaStream_t stream, bool pdl, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// One-time opt-in to large dynamic shared memory, per kernel (one `done` word each) and device.
+template <typename Kern>
+static cudaError_t allow_smem(Kern kern, std::atomic<unsigned>& done, int bytes = 227 * 1024) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned bit = 1u << (dev & 31);
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    else cudaGetLastError();                              // reported by the return value, not to the caller's next check
+    return e;
+}
+
+}  // namespace ztq

@@ -1,0 +1,112 @@
+// ztq_attn.cu -- extern "C" launchers of the attention over the paged 8-bit cache (see include/ztq.h).
+#include "../../include/ztq.h"
+
+#include "attn_q8.cuh"
+#include "launch.cuh"
+
+#include <cstdint>
+#include <cstring>
+
+namespace ztq {
+
+// Rows of a tile of attn_rows_kernel and its CTAs per SM: heads of 256 leave registers for eight rows only.
+static int attn_nt(int head_dim, long long rows) { return rows <= 8 || head_dim > 128 ? 1 : 2; }
+static int attn_ctas_per_sm(int head_dim, int nt, bool split) { return nt == 1 && head_dim <= 128 && !split ? 4 : head_dim <= 128 ? 2 : 1; }
+
+template <int D, int NT, bool SPLIT>
+static cudaError_t launch_rows(const AttnParams& p, int sms, cudaStream_t stream, bool pdl) {
+    const int grid = sms * attn_ctas_per_sm(D, NT, SPLIT);
+    static std::atomic<unsigned> done{0};
+    auto kern = attn_rows_kernel<D, NT, SPLIT>;
+    if (cudaError_t e = allow_smem(kern, done, 200 * 1024)) return e;
+    const size_t upto = (size_t)p.seqs * 8;
+    cudaError_t e = launch(kern, dim3(grid), dim3(kAttnThreads), kAttnWarps * 8 * NT * (D + 4) * 4 + upto, stream, pdl, p);
+    if (e != cudaSuccess) return e;
+    e = launch(attn_join_kernel<D, NT>, dim3(grid - 1), dim3(256), upto, stream, pdl, p, grid);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <int D>
+static cudaError_t launch_dim(const AttnParams& p, int nt, bool split, int sms, cudaStream_t stream, bool pdl) {
+    if constexpr (D <= 128) {
+        if (nt == 2) return split ? launch_rows<D, 2, true>(p, sms, stream, pdl) : launch_rows<D, 2, false>(p, sms, stream, pdl);
+    }
+    return split ? launch_rows<D, 1, true>(p, sms, stream, pdl) : launch_rows<D, 1, false>(p, sms, stream, pdl);
+}
+
+static int attn_block_shift(int block_size) {
+    for (int s = 4; s <= 7; ++s)
+        if (block_size == 1 << s) return s;
+    return -1;
+}
+
+}  // namespace ztq
+
+using namespace ztq;
+
+extern "C" {
+
+int ztq_take_error_attn() { return take_error(); }
+
+size_t ztq_attn_q8_workspace_bytes(int tokens, int sequences, int max_new, int q_heads, int kv_heads, int head_dim) {
+    if (tokens < 0 || sequences <= 0 || max_new <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads) return 0;
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
+    const int sms = device_info().sms > 0 ? device_info().sms : 148;
+    const int nt = attn_nt(head_dim, (long long)max_new * (q_heads / kv_heads));
+    return (size_t)sms * attn_ctas_per_sm(head_dim, nt, false) * 2 * 8 * nt * (head_dim + 2) * sizeof(float);
+}
+
+cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_head, long long y_token, long long y_head, int tokens, int q_heads,
+                        const int* query_start, const int* kv_len, const int* block_table, int sequences, int table_width, int max_new, int window,
+                        unsigned scale_bits, const ZtqKvCache* cache, void* workspace, size_t workspace_bytes, int flags, cudaStream_t stream) {
+    if (!q || !y || !query_start || !kv_len || !block_table || !cache || !cache->k || !cache->v || !cache->k_scale || !cache->v_scale || !workspace) return cudaErrorInvalidValue;
+    const int shift = attn_block_shift(cache->block_size), dim = cache->head_dim;
+    if (shift < 0 || (dim != 64 && dim != 128 && dim != 256) || cache->blocks <= 0 || cache->kv_heads <= 0) return cudaErrorInvalidValue;
+    if (cache->block_stride < (long long)cache->kv_heads * cache->block_size * dim || cache->block_stride % 16) return cudaErrorInvalidValue;
+    if (((uintptr_t)cache->k | (uintptr_t)cache->v | (uintptr_t)workspace) & 15) return cudaErrorInvalidValue;
+    if (tokens < 0 || q_heads <= 0 || q_heads % cache->kv_heads || sequences <= 0 || sequences > kAttnMaxSeqs || table_width <= 0 || max_new <= 0 || window < 0)
+        return cudaErrorInvalidValue;
+    if ((long long)table_width << shift > 0x7fffffffll || (long long)max_new * (q_heads / cache->kv_heads) > 0x7fffffffll) return cudaErrorInvalidValue;
+    if (flags & ~(ZTQ_X_F32 | ZTQ_Y_F32 | ZTQ_NO_PDL)) return cudaErrorInvalidValue;
+    if (workspace_bytes < ztq_attn_q8_workspace_bytes(tokens, sequences, max_new, q_heads, cache->kv_heads, dim)) return cudaErrorInvalidValue;
+    float scale;
+    memcpy(&scale, &scale_bits, 4);
+    const DeviceInfo dev = device_info();
+    if (dev.major < 10) return cudaErrorNoKernelImageForDevice;
+    if (tokens == 0) return cudaSuccess;
+    AttnParams p = {};
+    p.q = q;
+    p.y = y;
+    p.q_token = q_token; p.q_head = q_head; p.y_token = y_token; p.y_head = y_head;
+    p.query_start = query_start;
+    p.kv_len = kv_len;
+    p.block_table = block_table;
+    p.kc = static_cast<const int8_t*>(cache->k);
+    p.vc = static_cast<const int8_t*>(cache->v);
+    p.ks = cache->k_scale;
+    p.vs = cache->v_scale;
+    p.block_stride = cache->block_stride;
+    p.parts = static_cast<float*>(workspace);
+    p.seqs = sequences;
+    p.tokens = tokens;
+    p.max_new = max_new;
+    p.q_heads = q_heads;
+    p.kv_heads = cache->kv_heads;
+    p.group = q_heads / cache->kv_heads;
+    p.width = table_width;
+    p.shift = shift;
+    p.blocks = cache->blocks;
+    p.window = window;
+    p.scale_log2 = scale * 1.44269504088896340736f;
+    p.x_f32 = (flags & ZTQ_X_F32) ? 1 : 0;
+    p.y_f32 = (flags & ZTQ_Y_F32) ? 1 : 0;
+    p.vec = ((uintptr_t)q & 7) == 0 && q_token % 4 == 0 && q_head % 4 == 0;
+    p.min_rows = 1;
+    p.max_rows = 0x7fffffff;
+    const int nt = attn_nt(dim, (long long)max_new * p.group);
+    const bool split = p.x_f32 || p.y_f32, pdl = !(flags & ZTQ_NO_PDL);
+    return dim == 64 ? launch_dim<64>(p, nt, split, dev.sms, stream, pdl)
+         : dim == 128 ? launch_dim<128>(p, nt, split, dev.sms, stream, pdl) : launch_dim<256>(p, nt, split, dev.sms, stream, pdl);
+}
+
+}  // extern "C"

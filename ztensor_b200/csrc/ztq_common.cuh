@@ -19,11 +19,23 @@ enum : int {
     ZTQ_ERR_EMPTY_WAIT = 2,   // producer gave up waiting for a free stage
     ZTQ_ERR_TMEM_WAIT = 3,    // epilogue gave up waiting for the tensor pipe
     ZTQ_ERR_FLAG_WAIT = 4,    // all-reduce gave up waiting for a peer's flag
+    ZTQ_ERR_SLOT = 5,         // cache append: a slot outside the cache, or a block's rows out of order (row skipped)
+    ZTQ_ERR_POSITION = 6,     // rotary: a position outside the table (row becomes NaN)
+    ZTQ_ERR_BLOCK = 7,        // attention: a block table entry outside the cache (its tokens are not seen)
+    ZTQ_ERR_LENGTH = 8,       // attention: a sequence with more new tokens than announced (left out)
 };
 
-__device__ int g_ztq_error = 0;   // the library is a single translation unit
+static __device__ int g_ztq_error = 0;   // one word per translation unit; ztq_device_error() looks at all of them
 
 __device__ __forceinline__ void report_error(int code) { atomicCAS(&g_ztq_error, 0, code); }
+
+// Reads and clears the word of the translation unit that calls it (the device is idle).
+static inline int take_error() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_ztq_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v != 0) cudaMemcpyToSymbol(g_ztq_error, &zero, sizeof(int));
+    return v;
+}
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));

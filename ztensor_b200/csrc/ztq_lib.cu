@@ -9,48 +9,17 @@
 #include "gemv_stream.cuh"
 #include "gemv_w4pair.cuh"
 #include "gemm_w4g_tc.cuh"
+#include "launch.cuh"
 #include "ztq_common.cuh"
 
 #include <atomic>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <vector>
 
 namespace ztq {
-
-
-static inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
-
-struct DeviceInfo {
-    int sms = 0;
-    int major = 0;
-};
-
-static DeviceInfo device_info() {
-    // Queried per call: cheap attribute reads, no cached mutable state.
-    DeviceInfo d;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return d;
-    cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
-    cudaDeviceGetAttribute(&d.major, cudaDevAttrComputeCapabilityMajor, dev);
-    return d;
-}
-
-template <typename Kern, typename... Args>
-static cudaError_t launch(Kern kern, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, args...);
-}
 
 // ---------------------------------------------------------------------------
 // Launch plan of the streaming GEMV.
@@ -411,6 +380,11 @@ static cudaError_t gemv_kquant(const void* w_sep, long long data_offset, const v
 }  // namespace ztq
 
 using namespace ztq;
+
+extern "C" {
+int ztq_take_error_step();
+int ztq_take_error_attn();
+}
 
 // ---- batch >= 16: W4A16 skinny GEMM on tcgen05 / TMEM -------------------------------
 namespace {
@@ -1263,11 +1237,10 @@ int ztq_check_sm100(void) { return device_info().major == 10 ? 1 : 0; }
 int ztq_abi_version(void) { return 1; }
 
 int ztq_device_error(void) {
-    int v = 0, zero = 0;
     if (cudaDeviceSynchronize() != cudaSuccess) return -1;
-    if (cudaMemcpyFromSymbol(&v, g_ztq_error, sizeof(int)) != cudaSuccess) return -1;
-    if (v != 0) cudaMemcpyToSymbol(g_ztq_error, &zero, sizeof(int));
-    return v;
+    for (auto take : {&take_error, &ztq_take_error_step, &ztq_take_error_attn})   // one word per translation unit
+        if (int e = take()) return e;
+    return 0;
 }
 
 }  // extern "C"

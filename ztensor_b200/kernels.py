@@ -28,7 +28,7 @@ def _ptr(t):
 
 def _stream(stream):
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())     # torch.cuda.current_stream() without its objects
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
@@ -252,3 +252,175 @@ def describe_plan(fmt: str, n: int, k: int, batch: int = 1, group: int = 128, sm
     return dict(kernel=("plain", "stream", "pair")[v[0]], rows_per_launch=v[1], rt=v[2], rows_per_stage=v[3], stages=v[4],
                 overlay_stages=v[5], rows_per_pass=v[6], grid=v[7], tiles_per_cta=v[8], passes_per_cta=v[9],
                 warps_per_team=v[10], teams=v[11])
+
+
+# ---- the decode step around the projections: plan, rotary positions + 8-bit cache, attention, sampling.  Tensors carry
+# shapes, strides and types, so these wrappers check them here; X_F32 / Y_F32 follow from the dtypes.
+
+ROPE_PAIRS = 128
+ROPE_SCALING = {"none": 0, "linear": 1, "by_turns": 2, "by_dim": 3}
+SAMPLE_MAX_VOCAB = 389120
+
+
+def _arg(t, dtype, shape, name):
+    """Device pointer of a contiguous tensor of this type and shape on the current device."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous {dtype} {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}")
+    if not t.is_cuda or t.get_device() != _device():
+        raise ValueError(f"{name}: a tensor on the current CUDA device expected, got one on {t.device}")
+    return t.data_ptr()
+
+
+def _device():
+    return torch._C._cuda_getDevice()
+
+
+def _here(t, name):
+    if not t.is_cuda or t.get_device() != _device():
+        raise ValueError(f"{name}: a tensor on the current CUDA device expected, got one on {t.device}")
+    return t.data_ptr()
+
+
+def _heads(t, name):
+    """(pointer, token stride, head stride, is float32) of a [tokens, heads, dim] tensor with contiguous heads."""
+    f32 = t.dtype is torch.float32
+    strides = t.stride()
+    if len(strides) != 3 or not (f32 or t.dtype is torch.float16) or strides[2] != 1:
+        raise ValueError(f"{name}: float16 or float32 [tokens, heads, dim] with contiguous dim expected, got {t.dtype} {tuple(t.shape)}, strides {strides}")
+    return _here(t, name), strides[0], strides[1], f32
+
+
+class ZtqKvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("block_stride", C.c_longlong),
+                ("blocks", C.c_int), ("kv_heads", C.c_int), ("block_size", C.c_int), ("head_dim", C.c_int)]
+
+
+class ZtqRopeSpec(C.Structure):
+    _fields_ = [("base", C.c_double), ("factor", C.c_double), ("turns_low", C.c_double), ("turns_high", C.c_double),
+                ("original_positions", C.c_double), ("magnitude", C.c_double), ("rot_dim", C.c_int), ("scaling", C.c_int)]
+
+
+class KvCache:
+    """One layer's paged 8-bit cache: k, v int8 [blocks, kv_heads, block_size, head_dim] (the block stride is free, the rest
+    contiguous), k_scale, v_scale float32 [blocks, kv_heads].  Keeps the tensors alive and their description ready."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        blocks, heads, size, dim = k.shape
+        for t, name in ((k, "k"), (v, "v")):
+            if t.dtype is not torch.int8 or t.shape != k.shape or t.stride()[1:] != (size * dim, dim, 1) or t.stride(0) != k.stride(0):
+                raise ValueError(f"{name}: int8 [blocks, kv_heads, block_size, head_dim] with contiguous blocks expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}")
+        for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            _arg(t, torch.float32, (blocks, heads), name)
+        self.tensors = (k, v, k_scale, v_scale)
+        self.blocks, self.kv_heads, self.block_size, self.head_dim = blocks, heads, size, dim
+        self.desc = ZtqKvCache(_here(k, "k"), _here(v, "v"), k_scale.data_ptr(), v_scale.data_ptr(), k.stride(0) if blocks > 1 else heads * size * dim, blocks, heads, size, dim)
+        self.ptr = C.addressof(self.desc)
+
+    @classmethod
+    def empty(cls, blocks, kv_heads, block_size, head_dim, device="cuda"):
+        """A cache of its own memory; nothing in it needs a start value."""
+        k, v = (torch.empty(blocks, kv_heads, block_size, head_dim, dtype=torch.int8, device=device) for _ in range(2))
+        return cls(k, v, *(torch.zeros(blocks, kv_heads, device=device) for _ in range(2)))
+
+    def _on(self):
+        _here(self.tensors[0], "cache")
+        return self.ptr
+
+
+def kv_plan(ctx_len, new_len, block_table, ring, ring_state, ring_state_out, next_len, kv_len, query_start, positions, slots, status, block_size, flags=0, stream=None):
+    """The plan of a step: block table, slots, positions and lengths from the sequences' lengths (ztq_kv_plan).
+    All int32; next_len may be ctx_len and ring_state_out may be ring_state."""
+    i, n, rows = torch.int32, ctx_len.shape[0], slots.shape[0]
+    _lib.check(_lib.lib().ztq_kv_plan(
+        _arg(ctx_len, i, (n,), "ctx_len"), _arg(new_len, i, (n,), "new_len"), _arg(block_table, i, (n, block_table.shape[-1]), "block_table"), _arg(ring, i, (ring.numel(),), "ring"),
+        _arg(ring_state, i, (2,), "ring_state"), _arg(ring_state_out, i, (2,), "ring_state_out"), _arg(next_len, i, (n,), "next_len"), _arg(kv_len, i, (n,), "kv_len"),
+        _arg(query_start, i, (n + 1,), "query_start"), _arg(positions, i, (rows,), "positions"), _arg(slots, i, (rows,), "slots"), _arg(status, i, (n,), "status"),
+        n, block_table.shape[1], block_size, ring.shape[0], rows, flags, _stream(stream)), "ztq_kv_plan")
+
+
+def rope_table(rows, rot_dim, base, first=0, scaling="none", factor=1.0, turns_low=1.0, turns_high=4.0, original_positions=0, magnitude=1.0, out=None, flags=0, stream=None):
+    """{cos, sin} of positions first .. first + rows - 1, float32 [rows, rot_dim / 2, 2] (ztq_rope_table)."""
+    if scaling not in ROPE_SCALING:
+        raise ValueError(f"scaling: one of {sorted(ROPE_SCALING)} expected, got {scaling!r}")
+    if out is None:
+        out = torch.empty(rows, rot_dim // 2, 2, dtype=torch.float32, device="cuda")
+    spec = ZtqRopeSpec(base, factor, turns_low, turns_high, original_positions, magnitude, rot_dim, ROPE_SCALING[scaling])
+    _lib.check(_lib.lib().ztq_rope_table(_arg(out, torch.float32, (rows, rot_dim // 2, 2), "out"), first, rows, C.addressof(spec), flags, _stream(stream)), "ztq_rope_table")
+    return out
+
+
+def rope(x, y, table, positions, flags=0, stream=None):
+    """y = x [tokens, heads, dim] rotated to `positions`; y may be x (ztq_rope)."""
+    xp, xt, xh, xf = _heads(x, "x")
+    yp, yt, yh, yf = _heads(y, "y")
+    n, heads, dim = x.shape
+    if y.shape != x.shape:
+        raise ValueError(f"y: {tuple(x.shape)} expected, got {tuple(y.shape)}")
+    _lib.check(_lib.lib().ztq_rope(xp, yp, n, heads, dim, xt, xh, yt, yh, _arg(table, torch.float32, (*table.shape[:2], 2), "table"), table.shape[0], 2 * table.shape[1],
+                                   _arg(positions, torch.int32, (n,), "positions"), flags | (X_F32 if xf else 0) | (Y_F32 if yf else 0), _stream(stream)), "ztq_rope")
+
+
+def rope_append_q8(q, k, v, q_out, slots, cache, table=None, positions=None, flags=0, stream=None):
+    """Rotates q [tokens, q_heads, dim] into q_out (both may be None, or q_out may be q) and appends k (rotated), v [tokens, kv_heads, dim] to
+    the cache at `slots` (ztq_rope_append_q8).  table None: nothing is rotated.  flags: ROPE_PAIRS, NO_PDL."""
+    kp, kt, kh, xf = _heads(k, "k")
+    vp, vt, vh, vf = _heads(v, "v")
+    n = k.shape[0]
+    if k.shape != (n, cache.kv_heads, cache.head_dim) or v.shape != k.shape or vf != xf:
+        raise ValueError(f"k, v: one type and {(n, cache.kv_heads, cache.head_dim)} expected, got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
+    qp = qo = qt = qh = ot = oh = heads = 0
+    of = False
+    if q is not None:
+        qp, qt, qh, qf = _heads(q, "q")
+        qo, ot, oh, of = _heads(q_out, "q_out")
+        heads = q.shape[1]
+        if qf != xf or q.shape[0] != n or q.shape[2] != cache.head_dim or q_out.shape != q.shape:
+            raise ValueError(f"q, q_out: {n} rows of heads of {cache.head_dim} and the type of k expected, got {q.dtype} {tuple(q.shape)} and {tuple(q_out.shape)}")
+    tp = pp = rows = rot = 0
+    if table is not None:
+        tp, rows, rot = _arg(table, torch.float32, (*table.shape[:2], 2), "table"), table.shape[0], 2 * table.shape[1]
+        pp = _arg(positions, torch.int32, (n,), "positions")
+    _lib.check(_lib.lib().ztq_rope_append_q8(qp, kp, vp, qo, qt, qh, kt, kh, vt, vh, ot, oh, n, heads, tp, rows, rot, pp, _arg(slots, torch.int32, (n,), "slots"),
+                                             cache._on(), flags | (X_F32 if xf else 0) | (Y_F32 if of else 0), _stream(stream)), "ztq_rope_append_q8")
+
+
+def kv_read_q8(cache, slots, k_out, v_out, flags=0, stream=None):
+    """The cache's rows at `slots`, dequantized into k_out and v_out [tokens, kv_heads, dim] (either may be None) (ztq_kv_read_q8)."""
+    out = k_out if k_out is not None else v_out
+    if out is None or (out.dtype is not torch.float16 and out.dtype is not torch.float32):
+        raise ValueError("k_out, v_out: at least one float16 or float32 tensor expected")
+    shape = (slots.shape[0], cache.kv_heads, cache.head_dim)
+    kp, vp = (0 if t is None else _arg(t, out.dtype, shape, name) for t, name in ((k_out, "k_out"), (v_out, "v_out")))
+    _lib.check(_lib.lib().ztq_kv_read_q8(cache._on(), _arg(slots, torch.int32, shape[:1], "slots"), shape[0], kp, vp, flags | (Y_F32 if out.dtype is torch.float32 else 0),
+                                         _stream(stream)), "ztq_kv_read_q8")
+
+
+def attn_q8_workspace_bytes(tokens, sequences, max_new, q_heads, kv_heads, head_dim) -> int:
+    return int(_lib.lib().ztq_attn_q8_workspace_bytes(tokens, sequences, max_new, q_heads, kv_heads, head_dim))
+
+
+def attn_q8(q, y, query_start, kv_len, block_table, cache, workspace, max_new, scale, window=0, flags=0, stream=None):
+    """Causal attention of q [tokens, q_heads, dim] over the cache into y (ztq_attn_q8); window 0: all earlier positions."""
+    qp, qt, qh, xf = _heads(q, "q")
+    yp, yt, yh, yf = _heads(y, "y")
+    n, heads, dim = q.shape
+    seqs = kv_len.shape[0]
+    if y.shape != q.shape or dim != cache.head_dim:
+        raise ValueError(f"q, y: one shape and heads of {cache.head_dim} expected, got {tuple(q.shape)} and {tuple(y.shape)}")
+    i = torch.int32
+    _lib.check(_lib.lib().ztq_attn_q8(
+        qp, yp, qt, qh, yt, yh, n, heads, _arg(query_start, i, (seqs + 1,), "query_start"), _arg(kv_len, i, (seqs,), "kv_len"), _arg(block_table, i, (seqs, block_table.shape[-1]), "block_table"),
+        seqs, block_table.shape[1], max_new, window, C.c_uint.from_buffer(C.c_float(scale)).value, cache._on(), _here(workspace, "workspace"), workspace.numel() * workspace.element_size(),
+        flags | (X_F32 if xf else 0) | (Y_F32 if yf else 0), _stream(stream)), "ztq_attn_q8")
+
+
+def sample(logits, uniform, token, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None, flags=0, stream=None):
+    """One token per row of logits [rows, vocab] from `uniform` [rows] in [0, 1) (ztq_sample)."""
+    if logits.dim() != 2 or (logits.dtype is not torch.float16 and logits.dtype is not torch.float32) or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError(f"logits: float16 or float32 [rows, vocab] with contiguous rows expected, got {logits.dtype} {tuple(logits.shape)}, strides {logits.stride()}")
+    n, vocab = logits.shape
+    f, i = torch.float32, torch.int32
+    opt = lambda t, dtype, name: 0 if t is None else _arg(t, dtype, (n,), name)  # noqa: E731
+    _lib.check(_lib.lib().ztq_sample(_here(logits, "logits"), logits.stride(0) if n > 1 else 0, n, vocab, opt(temperature, f, "temperature"), opt(top_k, i, "top_k"), opt(top_p, f, "top_p"),
+                                     opt(min_p, f, "min_p"), _arg(uniform, f, (n,), "uniform"), _arg(token, i, (n,), "token"), opt(logprob, f, "logprob"),
+                                     flags | (X_F32 if logits.dtype is torch.float32 else 0), _stream(stream)), "ztq_sample")
