@@ -476,39 +476,70 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 && !SPLIT ? 
     }
 }
 
-// Adds the parts of the items that several CTAs shared.  CTA j of this grid looks at the boundary between the ranges of
-// CTAs j and j + 1 of attn_rows_kernel and does the item it cuts, if it is the first boundary inside that item.
+// Adds the parts of the items that several CTAs shared.  blockIdx.x = j looks at the boundary between the ranges of CTAs j
+// and j + 1 of attn_rows_kernel and does the item it cuts, if it is the first boundary inside that item; blockIdx.y is the
+// row.  A short row of long loads: the parts' maxima and sums are fetched together, then every warp adds its share of the
+// parts (all loads independent), then the warps' sums are added in order.
+constexpr int kJoinThreads = 256;
 template <int D, int NT>
-__global__ void __launch_bounds__(256) attn_join_kernel(const AttnParams p, int grid) {
-    constexpr int TILE = 8 * NT;
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnParams p, int grid) {
+    constexpr int TILE = 8 * NT, V = D / 32, WARPS = kJoinThreads / 32;   // V: dims per lane
     extern __shared__ __align__(16) uint8_t smem[];
     long long* upto = reinterpret_cast<long long*>(smem);
-    __shared__ long long part[8];
+    float* fix = reinterpret_cast<float*>(upto + p.seqs);                  // [parts], at most one per CTA
+    __shared__ long long part[WARPS];
+    __shared__ float red[WARPS][D + 1];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     grid_dep_launch();
     grid_dep_wait();
     attn_scan(p, TILE, upto, part);
     const long long total = upto[p.seqs - 1];
-    const int ctas = attn_ctas(total, grid), cta = blockIdx.x;
+    const int ctas = attn_ctas(total, grid), cta = blockIdx.x, r = blockIdx.y;
     if (cta + 1 >= ctas) return;
     const long long w = attn_cut(total, cta + 1, ctas);
     AttnSeq s;
     const AttnItem it = attn_find(p, TILE, upto, w, s);
-    if (it.begin == w || attn_cut(total, cta, ctas) > it.begin) return;     // no cut inside, or not the first one
-    int end = cta + 1;                                                      // CTAs cta .. end hold parts
-    while (attn_cut(total, end + 1, ctas) < it.begin + it.steps) ++end;
-    const int rows = it.r1 - it.r0;
-    for (int i = threadIdx.x; i < rows * D; i += blockDim.x) {
-        const int r = i / D, d = i % D;
-        float top = -INFINITY, sum = 0.f, v = 0.f;
-        for (int u = cta; u <= end; ++u) {
-            const float* row = p.parts + ((long long)u * 2 + (u == cta ? 1 : 0)) * TILE * (D + 2) + r * (D + 2);
-            const float m = row[D];
-            const float up = fmaxf(top, m), old = top == -INFINITY ? 0.f : exp2f(top - up), fix = m == -INFINITY ? 0.f : exp2f(m - up);
-            sum = old * sum + fix * row[D + 1];
-            v = old * v + fix * row[d];
-            top = up;
-        }
-        attn_store(p, s, it.r0 + r, it.h, d, sum > 0.f || sum != sum ? v / sum : 0.f);
+    if (it.begin == w || attn_cut(total, cta, ctas) > it.begin || r >= it.r1 - it.r0) return;     // no cut inside, or not the first one
+    // CTAs cta .. cta + n - 1 hold parts; the last is the one whose range reaches the item's end
+    const long long end = it.begin + it.steps;
+    int last = (int)(end * ctas / total);
+    while (last > cta && attn_cut(total, last, ctas) >= end) --last;
+    while (attn_cut(total, last + 1, ctas) < end) ++last;
+    const int n = last - cta + 1;
+    auto row_of = [&](int u) { return p.parts + ((long long)(cta + u) * 2 + (u == 0 ? 1 : 0)) * TILE * (D + 2) + r * (D + 2); };
+    float top = -INFINITY;
+    for (int u = tid; u < n; u += kJoinThreads) {
+        const float m = row_of(u)[D];
+        fix[u] = m;
+        top = fmaxf(top, m);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) red[warp][0] = top;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) top = fmaxf(top, red[k][0]);
+    __syncthreads();
+    float sum = 0.f, v[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = 0.f;
+#pragma unroll 4
+    for (int u = warp; u < n; u += WARPS) {
+        const float* row = row_of(u);
+        const float f = fix[u] == -INFINITY ? 0.f : exp2f(fix[u] - top);
+        sum += f * row[D + 1];
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] += f * row[32 * k + lane];
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) red[warp][32 * k + lane] = v[k];
+    if (lane == 0) red[warp][D] = sum;
+    __syncthreads();
+    for (int d = tid; d < D; d += kJoinThreads) {
+        float a = 0.f, b = 0.f;
+#pragma unroll
+        for (int k = 0; k < WARPS; ++k) { a += red[k][d]; b += red[k][D]; }
+        attn_store(p, s, it.r0 + r, it.h, d, b > 0.f || b != b ? a / b : 0.f);
     }
 }
 

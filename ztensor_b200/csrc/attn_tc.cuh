@@ -1,0 +1,521 @@
+// attn_tc.cuh -- the attention of attn_q8.cuh for sequences with many new tokens (prompts), on the tcgen05 tensor cores.
+//
+// An item is (sequence, 256 rows, kv head) and one CTA; its rows are two tiles of 128 (M of the products).  Per step of 128
+// keys:
+//   S_t = Q_t K^T   (fp16 x fp16 -> fp32 in TMEM, 128 columns)            Q_t, K from shared memory
+//   P_t = 2^(S_t f - m + lift) as fp16, over the columns of S_t
+//   O_t += P_t V    (P_t from TMEM, V^T from shared memory; D columns)
+// The codes become fp16 operands (exactly) on the way into shared memory, once per step for both tiles: a step's 64 KB of
+// operands cost what a quarter of the exponentials costs.  Within a step K codes are multiplied by their block's scale over
+// the step's largest, V codes by theirs over a power of two near the step's largest, so that one factor per step remains
+// (exact for the powers of two that the append writes; other scales are rounded to fp16).
+//
+// Roles of the 17 warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread is a row: TMEM lane), 8-15 codes -> operands
+// (warp w: keys 16 w .. 16 w + 15 of a step), 16 issues the products.  The two tiles alternate: while one is in its softmax
+// the tensor cores work for the other.  The running maximum moves only when a score exceeds it by more than kAttnSlack
+// (then the row's O is rescaled in TMEM), as does the reference of the V scales.
+// Operands stand in the canonical K-major layout without swizzle: core matrices of 8 rows x 16 bytes, 128 bytes apart along
+// the contraction; both store patterns below are free of bank conflicts.
+//
+// What bounds it: per step and SM 2048 clocks of tensor time, the same of exponentials (16 per clock) and the same of
+// shared-memory traffic; P is rounded to fp16 like the outputs.
+//
+// With few items the keys are cut into `splits` ranges of steps; a CTA then leaves {max, sum, rows} in the workspace and
+// attn_tc_join_kernel adds the ranges in order.
+#pragma once
+
+#include "attn_q8.cuh"
+#include "tc_common.cuh"
+
+namespace ztq {
+
+constexpr int kTcaRows = 256, kTcaKeys = 128;
+constexpr int kTcaThreads = 17 * 32;
+constexpr float kTcaLift = 5.f;                 // with kAttnSlack and kTcaScaleSlack: P < 2^15
+constexpr int kTcaScaleSlack = 2;
+
+struct TcaInfo {                                // one step's factors
+    float kref;                                 // scores: S * kref
+    int vexp;                                   // V operand = value / 2^vexp
+    uint32_t hidden, bad_v;                     // groups of 16 keys without a block; with a V scale that is not finite
+};
+
+struct TcaShared {
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], info_full[4];
+    TcaInfo info[4];
+    uint32_t tmem;
+};
+template <int D>
+__host__ __device__ constexpr int tca_smem() {
+    const int n = kTcaRows * D * 2 + 4 * kTcaKeys * D * 2 + 1024;
+    return n < 120 * 1024 ? 120 * 1024 : n;     // one CTA per SM: it holds all of TMEM
+}
+
+struct TcaParams {
+    AttnParams a;
+    int splits;
+    float* parts;                               // [item][split][256][D + 2]
+};
+
+struct TcaItem {
+    int b, r0, r1, h, lo, hi;
+    AttnSeq s;
+};
+// upto[b]: row pairs of sequences 0 .. b
+__device__ __forceinline__ void tca_scan(const AttnParams& p, int* upto, int* part) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int before = 0;
+    for (int b0 = 0; b0 < p.seqs; b0 += blockDim.x) {
+        const int b = b0 + threadIdx.x;
+        int v = b < p.seqs ? (attn_seq(p, b).rows(p.group) + kTcaRows - 1) / kTcaRows : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        __syncthreads();
+        if (lane == 31) part[warp] = v;
+        __syncthreads();
+        int all = before;
+        for (int w = 0; w < warps; ++w) {
+            if (w < warp) v += part[w];
+            all += part[w];
+        }
+        if (b < p.seqs) upto[b] = before + v;
+        before = all;
+    }
+    __syncthreads();
+}
+// Item i, or false behind the last.  Within a sequence the items with most keys come first: the hardware deals CTAs in
+// order, so the short ones fill the end.
+__device__ __forceinline__ bool tca_item(const AttnParams& p, const int* upto, long long i, TcaItem& it) {
+    const int pair = (int)(i / p.kv_heads);
+    it.h = (int)(i % p.kv_heads);
+    if (pair >= upto[p.seqs - 1]) return false;
+    int lo = 0, hi = p.seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (upto[mid] > pair) hi = mid; else lo = mid + 1;
+    }
+    it.b = lo;
+    it.s = attn_seq(p, lo);
+    const int rows = it.s.rows(p.group);
+    it.r0 = (upto[lo] - 1 - pair) * kTcaRows;
+    it.r1 = min(it.r0 + kTcaRows, rows);
+    attn_span(p, it.s, it.r0, it.r1, it.lo, it.hi);
+    return true;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Four biased codes -> two pairs of fp16, times r where the group has a factor.
+__device__ __forceinline__ uint32_t scaled(uint32_t x, bool plain, __half2 r) {
+    const uint32_t u = unbias(x);
+    if (plain) return u;
+    const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&u), r);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams tp) {
+    constexpr int CG = D / 8;                               // 16-byte columns of a K-major row of D
+    constexpr int QB = 128 * D * 2, KB = kTcaKeys * D * 2;  // bytes of a tile of Q, of a K or V operand
+    constexpr uint32_t kS = 0, kO = 256;                    // TMEM columns of the score tiles and of the outputs
+    extern __shared__ __align__(1024) uint8_t smem_tc[];
+    uint8_t* sq = smem_tc;
+    uint8_t* sk = smem_tc + 2 * QB;
+    uint8_t* sv = sk + 2 * KB;
+    TcaShared& sh = *reinterpret_cast<TcaShared*>(sv + 2 * KB);
+    const AttnParams& p = tp.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+    grid_dep_launch();
+    grid_dep_wait();
+    // the scan's scratch lies where the operands will be
+    int* upto = reinterpret_cast<int*>(sk);
+    tca_scan(p, upto, reinterpret_cast<int*>(sv));
+    TcaItem it;
+    const bool mine = tca_item(p, upto, blockIdx.x, it);
+    __syncthreads();
+    if (!mine) return;
+    const int kt_lo = it.lo / kTcaKeys, kt_all = max(0, (it.hi + kTcaKeys - 1) / kTcaKeys - kt_lo);
+    const int kt0 = kt_lo + (int)((long long)kt_all * blockIdx.y / tp.splits), kt1 = kt_lo + (int)((long long)kt_all * (blockIdx.y + 1) / tp.splits);
+    const int n = kt1 - kt0, rows = it.r1 - it.r0, tiles = rows > 128 ? 2 : 1;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.k_full[i], 8); mbar_init(&sh.k_empty[i], 1);
+            mbar_init(&sh.v_full[i], 8); mbar_init(&sh.v_empty[i], 1);
+            mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 128); mbar_init(&sh.o_full[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) mbar_init(&sh.info_full[i], 1);
+        mbar_fence_init();
+    }
+    if (warp == 16) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // queries: 16-byte pieces in K-major order, a phase of eight lanes writes eight rows of one column
+    for (int i = tid; i < tiles * 128 * CG; i += kTcaThreads) {
+        const int r = (i & 7) + (i >> 3) / CG * 8, col = (i >> 3) % CG, row = it.r0 + r;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < it.r1) {
+            const __half* src = static_cast<const __half*>(p.q) + (it.s.first + row / p.group) * p.q_token + (long long)(it.h * p.group + row % p.group) * p.q_head + 8 * col;
+            if (p.vec) {
+                const uint2 a = *reinterpret_cast<const uint2*>(src), b = *reinterpret_cast<const uint2*>(src + 4);
+                v = make_uint4(a.x, a.y, b.x, b.y);
+            } else {
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = (uint32_t)__half_as_ushort(src[2 * k]) | (uint32_t)__half_as_ushort(src[2 * k + 1]) << 16;
+                v = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            if (p.scale_log2 < 0) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }   // scores use |scale|
+        }
+        *reinterpret_cast<uint4*>(sq + (r >> 3) * (CG * 128) + col * 128 + (r & 7) * 16) = v;
+    }
+    proxy_fence_async();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int phase) {
+        if (ok && !mbar_wait(bar, phase & 1)) {
+            ok = false;
+            report_error(ZTQ_ERR_TMEM_WAIT);
+        }
+        return ok;
+    };
+
+    if (warp >= 8 && warp < 16) {
+        // ------------------------------------------------ codes -> operands
+        const int w = warp - 8;
+        const int* table = p.block_table + (long long)it.b * p.width;
+        constexpr int KL = D / 64, LR = D / 4, VG = LR / 16;      // 16-byte loads per key and lane; lanes per row of V, key groups per lane
+        const int vg = lane / LR, vd = lane % LR;                 // V: first key group, word of four dims
+        const int rot = (vd >> 1) & 3;
+        auto sel = [](int a, int b) { return (uint32_t)(a | (4 + a) << 4 | b << 8 | (4 + b) << 12); };
+        const uint32_t sel0 = sel(rot, (rot + 1) & 3), sel1 = sel((rot + 2) & 3, (rot + 3) & 3);
+        uint4 kb[2][KL];
+        uint32_t vb[VG][8];
+        float ks = 0.f, vs = 0.f;                                 // of group `lane & 7` of the step
+        int blk = -1;                                             // ditto
+        auto load = [&](int kt) {
+            // every lane looks up group (lane & 7): all groups' scales are known to all warps
+            const int tok = kt * kTcaKeys + 16 * (lane & 7);
+            blk = -1;
+            ks = vs = 0.f;
+            if (tok < it.hi) {
+                blk = table[tok >> p.shift];
+                if ((unsigned)blk >= (unsigned)p.blocks) {
+                    report_error(ZTQ_ERR_BLOCK);
+                    blk = -1;
+                } else {
+                    ks = p.ks[(long long)blk * p.kv_heads + it.h];
+                    vs = p.vs[(long long)blk * p.kv_heads + it.h];
+                }
+            }
+            const int own = __shfl_sync(0xffffffffu, blk, w);
+            const int at = (kt * kTcaKeys + 16 * w) & ((1 << p.shift) - 1);
+            const long long off = max(own, 0) * p.block_stride + (((long long)it.h << p.shift) + at) * D;
+            if (own >= 0) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < KL; ++j) kb[i][j] = ld_stream(p.kc + off + ((lane & 7) + 8 * i) * D + 16 * ((lane >> 3) + 4 * j));
+#pragma unroll
+                for (int g = 0; g < VG; ++g)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) vb[g][i] = __ldg(reinterpret_cast<const uint32_t*>(p.vc + off + (8 * (vg + g) + i) * D + 4 * vd));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < KL; ++j) kb[i][j] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int g = 0; g < VG; ++g)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) vb[g][i] = 0;
+            }
+        };
+        if (n > 0) load(kt0);
+        for (int i = 0; i < n; ++i) {
+            const int slot = i & 1;
+            // factors of the step
+            const bool fine_v = fabsf(vs) <= 3.402823466e38f;
+            float kref = fabsf(ks) <= 3.402823466e38f ? fabsf(ks) : 0.f;
+            uint32_t vtop = fine_v ? __float_as_uint(fabsf(vs)) >> 23 : 0u;
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) {
+                kref = fmaxf(kref, __shfl_xor_sync(0xffffffffu, kref, o));
+                vtop = max(vtop, __shfl_xor_sync(0xffffffffu, vtop, o));
+            }
+            if (!(kref > 0.f)) kref = 1.f;
+            const int vexp = vtop ? min(max((int)vtop - 127, -120), 120) : 0;
+            const uint32_t hidden = __ballot_sync(0xffffffffu, blk < 0) & 255u, bad_v = __ballot_sync(0xffffffffu, blk >= 0 && !fine_v) & 255u;
+            const float rk = __shfl_sync(0xffffffffu, ks, w) / kref;
+            const float rv = __shfl_sync(0xffffffffu, fine_v ? vs : 0.f, w) * __uint_as_float((uint32_t)(127 - vexp) << 23);
+            const bool plain_k = rk == 1.f, plain_v = rv == 1.f;
+            const __half2 hk = __float2half2_rn(rk), hv = __float2half2_rn(rv);
+            if (w == 0 && lane == 0) {
+                sh.info[i & 3] = TcaInfo{kref, vexp, hidden, bad_v};
+                mbar_arrive(&sh.info_full[i & 3]);
+            }
+            // K: key (lane & 7) + 8 a, columns 2 c and 2 c + 1 for the loaded piece c = lane / 8 + 4 j
+            if (i >= 2 && !wait(&sh.k_empty[slot], (i >> 1) - 1)) break;
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int j = 0; j < KL; ++j) {
+                    const uint32_t x[4] = {kb[a][j].x ^ 0x80808080u, kb[a][j].y ^ 0x80808080u, kb[a][j].z ^ 0x80808080u, kb[a][j].w ^ 0x80808080u};
+                    uint32_t o[8];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        o[2 * k] = scaled(__byte_perm(x[k], 0x64646464u, 0x4140), plain_k, hk);
+                        o[2 * k + 1] = scaled(__byte_perm(x[k], 0x64646464u, 0x4342), plain_k, hk);
+                    }
+                    uint8_t* d = sk + slot * KB + (2 * w + a) * (CG * 128) + 2 * ((lane >> 3) + 4 * j) * 128 + (lane & 7) * 16;
+                    *reinterpret_cast<uint4*>(d) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<uint4*>(d + 128) = make_uint4(o[4], o[5], o[6], o[7]);
+                }
+            proxy_fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.k_full[slot]);
+            // V transposed: eight keys of one dim are 16 bytes; the lane's four dims in an order that spreads the banks
+            if (i >= 2 && !wait(&sh.v_empty[slot], (i >> 1) - 1)) break;
+#pragma unroll
+            for (int g = 0; g < VG; ++g) {
+                uint32_t o[4][4];                                 // [dim slot][pair of keys]
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t x = vb[g][2 * k] ^ 0x80808080u, y = vb[g][2 * k + 1] ^ 0x80808080u;
+                    const uint32_t u = __byte_perm(x, y, sel0), v = __byte_perm(x, y, sel1);
+                    o[0][k] = scaled(__byte_perm(u, 0x64646464u, 0x4140), plain_v, hv);
+                    o[1][k] = scaled(__byte_perm(u, 0x64646464u, 0x4342), plain_v, hv);
+                    o[2][k] = scaled(__byte_perm(v, 0x64646464u, 0x4140), plain_v, hv);
+                    o[3][k] = scaled(__byte_perm(v, 0x64646464u, 0x4342), plain_v, hv);
+                }
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const int dim = 4 * vd + ((d + rot) & 3);
+                    *reinterpret_cast<uint4*>(sv + slot * KB + (dim >> 3) * (kTcaKeys / 8 * 128) + (2 * w + vg + g) * 128 + (dim & 7) * 16) = make_uint4(o[d][0], o[d][1], o[d][2], o[d][3]);
+                }
+            }
+            proxy_fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.v_full[slot]);
+            if (i + 1 < n) load(kt0 + i + 1);
+        }
+    } else if (warp == 16) {
+        // ------------------------------------------------ products
+        if (elect_one()) {
+            const uint32_t id_s = tc_idesc_f16(kTcaKeys), id_o = tc_idesc_f16(D);
+            auto scores = [&](int t, int i) {
+                const uint64_t a = tc_smem_desc(sq + t * QB, 128, CG * 128), b = tc_smem_desc(sk + (i & 1) * KB, 128, CG * 128);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) tc_mma_f16(tmem + kS + 128 * t, a + 16 * k, b + 16 * k, id_s, k > 0);
+                tc_commit(&sh.s_full[t]);
+            };
+            if (n > 0 && wait(&sh.k_full[0], 0)) {
+                tc_fence_after();
+                for (int t = 0; t < tiles; ++t) scores(t, 0);
+                tc_commit(&sh.k_empty[0]);
+            }
+            for (int i = 0; i < n && ok; ++i) {
+                if (!wait(&sh.v_full[i & 1], i >> 1)) break;
+                if (i + 1 < n && !wait(&sh.k_full[(i + 1) & 1], (i + 1) >> 1)) break;
+                for (int t = 0; t < tiles; ++t) {
+                    if (!wait(&sh.p_full[t], i)) break;
+                    tc_fence_after();
+                    const uint64_t b = tc_smem_desc(sv + (i & 1) * KB, 128, kTcaKeys / 8 * 128);
+#pragma unroll
+                    for (int k = 0; k < kTcaKeys / 16; ++k) tc_mma_f16_ta(tmem + kO + D * t, tmem + kS + 128 * t + 8 * k, b + 16 * k, id_o, i > 0 || k > 0);
+                    if (t == tiles - 1) tc_commit(&sh.v_empty[i & 1]);
+                    if (i + 1 < n) {
+                        scores(t, i + 1);
+                        if (t == tiles - 1) tc_commit(&sh.k_empty[(i + 1) & 1]);
+                    } else tc_commit(&sh.o_full[t]);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp < 8 && (warp >> 2) < tiles) {
+        // ------------------------------------------------ softmax: a thread is a row
+        const int t = warp >> 2, r = it.r0 + 128 * t + (warp & 3) * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);         // TMEM address: lane << 16 | column
+        const uint32_t s_at = lanes + kS + 128 * t, o_at = lanes + kO + D * t;
+        const bool live = r < it.r1;
+        const int base = it.s.len - it.s.fresh;
+        const int z = live ? min(base + r / p.group, it.s.len - 1) : -1;    // last key the row sees
+        const int z_lo = p.window > 0 ? z - p.window : -1;                  // the last one in front of those it sees
+        const float scale = fabsf(p.scale_log2);
+        float m = -INFINITY, l = 0.f;
+        int vrun = -1000;
+        for (int i = 0; i < n; ++i) {
+            if (!wait(&sh.info_full[i & 3], i >> 2) || !wait(&sh.s_full[t], i)) break;
+            tc_fence_after();
+            const TcaInfo info = sh.info[i & 3];
+            const float f = info.kref * scale;
+            const int key0 = (kt0 + i) * kTcaKeys;
+            // keys of the step that the row sees: columns (a, b], less hidden groups
+            const int a = z_lo - key0, b = z - key0;
+            const bool edge = __any_sync(0xffffffffu, a >= 0 || b < kTcaKeys - 1) || info.hidden;
+            auto seen = [&](int col) { return col <= b && col > a && !(info.hidden >> (col >> 4) & 1); };
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float s[32];
+                tc_ld32(s_at + 32 * c, s);
+                if (edge) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) top = seen(32 * c + k) ? fmaxf(top, s[k]) : top;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) top = fmaxf(top, fmaxf(s[k], s[k + 1]));
+                }
+            }
+            top = top == -INFINITY ? top : top * f;
+            const bool grows = top > m + kAttnSlack, scale_grows = info.vexp > vrun + kTcaScaleSlack;
+            if (__any_sync(0xffffffffu, grows) || scale_grows) {
+                const float m_new = fmaxf(m, top);
+                float fix = m == -INFINITY ? 0.f : ex2(m - m_new);
+                l *= fix;
+                if (scale_grows) {
+                    fix *= vrun > -1000 ? ex2((float)max(vrun - info.vexp, -126)) : 0.f;
+                    vrun = info.vexp;
+                }
+                if (i > 0) {
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        float o[32];
+                        tc_ld32(o_at + 32 * c, o);
+                        uint32_t u[16];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(o[16 * h + k] * fix);
+                            tc_st16(o_at + 32 * c + 16 * h, u);
+                        }
+                    }
+                }
+                m = m_new;
+            }
+            const float m_safe = m == -INFINITY ? 0.f : m, shift = kTcaLift + (float)max(info.vexp - vrun, -100) - m_safe;
+            float sum = 0.f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float s[32];
+                tc_ld32(s_at + 32 * c, s);
+                uint32_t u[16];
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                    float e0 = ex2(fmaf(s[k], f, shift)), e1 = ex2(fmaf(s[k + 1], f, shift));
+                    if (edge) {
+                        e0 = seen(32 * c + k) ? e0 : 0.f;
+                        e1 = seen(32 * c + k + 1) ? e1 : 0.f;
+                    }
+                    sum += e0;
+                    sum += e1;
+                    u[k >> 1] = pack_half2(e0, e1);
+                }
+                tc_st16(s_at + 16 * c, u);                      // over scores that were read
+            }
+            l = fmaf(sum, ex2((float)-max(info.vexp - vrun, -100)), l);
+            if (info.bad_v)
+                for (int g = 0; g < 8; ++g)                     // a V scale that is not finite: NaN for the rows that see its keys
+                    if (info.bad_v >> g & 1 && max(16 * g, a + 1) <= min(16 * g + 15, b)) l = __int_as_float(0x7fc00000);
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(&sh.p_full[t]);
+        }
+        if (n > 0 && wait(&sh.o_full[t], 0)) tc_fence_after();
+        // ---- the row's output, or its part
+        const float vref = n > 0 && vrun > -1000 ? ex2((float)vrun) : 0.f;
+        const float inv = l > 0.f || l != l ? vref / l : 0.f;
+        float* part = tp.parts + (((long long)blockIdx.x * tp.splits + blockIdx.y) * kTcaRows + (r - it.r0)) * (D + 2);
+        const long long to = live ? (it.s.first + r / p.group) * p.y_token + (long long)(it.h * p.group + r % p.group) * p.y_head : 0;
+        const bool wide = p.y_token % 8 == 0 && p.y_head % 8 == 0 && ((uintptr_t)p.y & 15) == 0;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            if (n > 0 && ok) tc_ld32(o_at + 32 * c, o);
+            else {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = 0.f;
+            }
+            if (!live || !ok) continue;
+            if (tp.splits > 1) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) *reinterpret_cast<float2*>(part + 32 * c + k) = make_float2(o[k] * vref, o[k + 1] * vref);
+            } else {
+                __half* y = static_cast<__half*>(p.y) + to + 32 * c;
+                if (wide) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8)
+                        *reinterpret_cast<uint4*>(y + k) = make_uint4(pack_half2(o[k] * inv, o[k + 1] * inv), pack_half2(o[k + 2] * inv, o[k + 3] * inv),
+                                                                      pack_half2(o[k + 4] * inv, o[k + 5] * inv), pack_half2(o[k + 6] * inv, o[k + 7] * inv));
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) y[k] = __float2half_rn(o[k] * inv);
+                }
+            }
+        }
+        if (live && ok && tp.splits > 1) { part[D] = m; part[D + 1] = l; }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 16) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// Adds the ranges of an item in order: a warp per row, blockIdx.x the item, blockIdx.y eight of its rows.
+template <int D>
+__global__ void __launch_bounds__(256) attn_tc_join_kernel(const TcaParams tp) {
+    extern __shared__ int tca_upto[];
+    __shared__ int part[8];
+    const AttnParams& p = tp.a;
+    grid_dep_launch();
+    grid_dep_wait();
+    tca_scan(p, tca_upto, part);
+    TcaItem it;
+    if (!tca_item(p, tca_upto, blockIdx.x, it)) return;
+    const int lane = threadIdx.x & 31, r = it.r0 + blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (r >= it.r1) return;
+    float top = -INFINITY;
+    auto row_of = [&](int u) { return tp.parts + (((long long)blockIdx.x * tp.splits + u) * kTcaRows + (r - it.r0)) * (D + 2); };
+    for (int u = 0; u < tp.splits; ++u) top = fmaxf(top, row_of(u)[D]);
+    float sum = 0.f, v[D / 32] = {};
+    for (int u = 0; u < tp.splits; ++u) {
+        const float* row = row_of(u);
+        const float fix = row[D] == -INFINITY ? 0.f : exp2f(row[D] - top);
+        sum += fix * row[D + 1];
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) v[k] += fix * row[32 * k + lane];
+    }
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) attn_store(p, it.s, r, it.h, 32 * k + lane, sum > 0.f || sum != sum ? v[k] / sum : 0.f);
+}
+
+}  // namespace ztq

@@ -2,8 +2,10 @@
 #include "../../include/ztq.h"
 
 #include "attn_q8.cuh"
+#include "attn_tc.cuh"
 #include "launch.cuh"
 
+#include <algorithm>
 #include <cstdint>
 #include <cstring>
 
@@ -22,7 +24,7 @@ static cudaError_t launch_rows(const AttnParams& p, int sms, cudaStream_t stream
     const size_t upto = (size_t)p.seqs * 8;
     cudaError_t e = launch(kern, dim3(grid), dim3(kAttnThreads), kAttnWarps * 8 * NT * (D + 4) * 4 + upto, stream, pdl, p);
     if (e != cudaSuccess) return e;
-    e = launch(attn_join_kernel<D, NT>, dim3(grid - 1), dim3(256), upto, stream, pdl, p, grid);
+    e = launch(attn_join_kernel<D, NT>, dim3(grid - 1, 8 * NT), dim3(kJoinThreads), upto + grid * sizeof(float), stream, pdl, p, grid);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -32,6 +34,44 @@ static cudaError_t launch_dim(const AttnParams& p, int nt, bool split, int sms, 
         if (nt == 2) return split ? launch_rows<D, 2, true>(p, sms, stream, pdl) : launch_rows<D, 2, false>(p, sms, stream, pdl);
     }
     return split ? launch_rows<D, 1, true>(p, sms, stream, pdl) : launch_rows<D, 1, false>(p, sms, stream, pdl);
+}
+
+// Prompts: sequences with more than kTcMinRows rows per kv head go to the tensor-core kernel (fp16, heads of 64 and 128).
+constexpr int kTcMinRows = 64;
+
+struct TcPlan {
+    long long items = 0;          // CTAs of one split; 0: the kernel is not used
+    int splits = 1;
+    size_t bytes = 0;             // of its workspace
+};
+static TcPlan tc_plan(int tokens, int sequences, long long most_rows, int group, int kv_heads, int head_dim, int sms) {
+    TcPlan t;
+    if (most_rows <= kTcMinRows || head_dim > 128) return t;
+    // an item is 256 rows of a sequence: full ones, and one begun by each sequence that has enough rows
+    const long long rows = (long long)tokens * group, full = rows / kTcaRows;
+    const long long begun = sequences == 1 ? 1 : std::min<long long>(sequences, rows / (kTcMinRows + 1) + 1);
+    t.items = (full + begun) * kv_heads;
+    // few items: cut their keys so that every SM has a CTA
+    const long long few = (full > 0 ? full : 1) * kv_heads;
+    if (few < sms) t.splits = (int)std::min<long long>(sms / few, 32);
+    if (t.splits > 1) t.bytes = (size_t)t.items * t.splits * kTcaRows * (head_dim + 2) * sizeof(float);
+    return t;
+}
+
+template <int D>
+static cudaError_t launch_tc(const AttnParams& p, const TcPlan& plan, cudaStream_t stream, bool pdl) {
+    TcaParams tp;
+    tp.a = p;
+    // a split is worth four steps
+    tp.splits = (int)std::max<long long>(1, std::min<long long>(plan.splits, (((long long)p.width << p.shift) + 4 * kTcaKeys - 1) / (4 * kTcaKeys)));
+    tp.parts = p.parts;
+    static std::atomic<unsigned> done{0};
+    auto kern = attn_tc_kernel<D>;
+    if (cudaError_t e = allow_smem(kern, done, tca_smem<D>())) return e;
+    cudaError_t e = launch(kern, dim3((unsigned)plan.items, tp.splits), dim3(kTcaThreads), tca_smem<D>(), stream, pdl, tp);
+    if (e != cudaSuccess) return e;
+    if (tp.splits > 1) e = launch(attn_tc_join_kernel<D>, dim3((unsigned)plan.items, kTcaRows / 8), dim3(256), p.seqs * sizeof(int), stream, pdl, tp);
+    return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 static int attn_block_shift(int block_size) {
@@ -51,9 +91,11 @@ int ztq_take_error_attn() { return take_error(); }
 size_t ztq_attn_q8_workspace_bytes(int tokens, int sequences, int max_new, int q_heads, int kv_heads, int head_dim) {
     if (tokens < 0 || sequences <= 0 || max_new <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads) return 0;
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
-    const int sms = device_info().sms > 0 ? device_info().sms : 148;
-    const int nt = attn_nt(head_dim, (long long)max_new * (q_heads / kv_heads));
-    return (size_t)sms * attn_ctas_per_sm(head_dim, nt, false) * 2 * 8 * nt * (head_dim + 2) * sizeof(float);
+    const int sms = device_info().sms > 0 ? device_info().sms : 148, group = q_heads / kv_heads;
+    const long long rows = (long long)max_new * group;
+    const int nt = attn_nt(head_dim, rows);
+    return std::max((size_t)sms * attn_ctas_per_sm(head_dim, nt, false) * 2 * 8 * nt * (head_dim + 2) * sizeof(float),
+                    tc_plan(tokens, sequences, rows, group, kv_heads, head_dim, sms).bytes);
 }
 
 cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_head, long long y_token, long long y_head, int tokens, int q_heads,
@@ -105,6 +147,18 @@ cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_h
     p.max_rows = 0x7fffffff;
     const int nt = attn_nt(dim, (long long)max_new * p.group);
     const bool split = p.x_f32 || p.y_f32, pdl = !(flags & ZTQ_NO_PDL);
+    if (!split) {
+        const TcPlan plan = tc_plan(tokens, sequences, (long long)max_new * p.group, p.group, p.kv_heads, dim, dev.sms);
+        if (plan.items > 0x7fffffff) return cudaErrorInvalidValue;
+        if (plan.items > 0) {
+            // a single sequence goes there whatever it turns out to bring; several are told apart on the device
+            if (sequences > 1) p.min_rows = kTcMinRows + 1;
+            cudaError_t e = dim == 64 ? launch_tc<64>(p, plan, stream, pdl) : launch_tc<128>(p, plan, stream, pdl);
+            if (e != cudaSuccess || sequences == 1) return e;
+            p.min_rows = 1;
+            p.max_rows = kTcMinRows;
+        }
+    }
     return dim == 64 ? launch_dim<64>(p, nt, split, dev.sms, stream, pdl)
          : dim == 128 ? launch_dim<128>(p, nt, split, dev.sms, stream, pdl) : launch_dim<256>(p, nt, split, dev.sms, stream, pdl);
 }
