@@ -7,37 +7,42 @@
 // attn_rows_kernel: a row is a (token, query head) pair; the rows of a sequence that share a kv head are multiplied
 // together, 8 NT of them at a time, so that a block of the cache is read once for all of them.  Bound by HBM while the
 // rows of an item fit one tile (decoding, drafts).
+//   One CTA per SM: a producer warp keeps a ring of steps of 128 tokens (32 KB at D = 128) filled by tiled TMA copies, one
+// per block, and looks up block table and scales one step ahead; eight warps take 16 tokens of each step.
 //   S^T = K Q^T and Y^T = V^T P^T by mma.sync m16n8k16 with the TOKENS (then the dims) as M and the rows as N = 8: a
 // decode step has 4 to 8 rows per kv head, which as M would waste half of every instruction and more.
-//   No shared memory on the way: the contraction index may be permuted as long as both operands agree, so every lane
-// loads 16 contiguous bytes of the cache at a time and has exactly the codes its fragments need.  K: lane (g, c) holds
-// tokens g and g + 8 and bytes 64 l + 16 c of each.  V: lane (g, c) holds tokens 2c, 2c + 1, 2c + 8, 2c + 9 and dims
-// g D/8 .. (g + 1) D/8, and pairs two tokens' codes by byte permutes.  P^T is the transposed accumulator of S^T
-// (movmatrix).  A code becomes fp16 exactly: 0x6400 | (code + 128) is 1152 + code.
+//   The contraction index may be permuted as long as both operands agree, so every lane reads 16 contiguous bytes of the
+// step at a time and has exactly the codes its fragments need.  K: lane (g, c) holds tokens tau(g) and tau(g) + 8 and the
+// 16-byte pieces c + 4 l of each.  V: lane (g, c) holds tokens tau(2c), tau(2c + 1) and those + 8, pieces g + 8 j, and
+// pairs two tokens' codes by byte permutes.  P^T is the transposed accumulator of S^T (movmatrix).  tau = 0 5 2 7 4 1 6 3:
+// with the copies' 128-byte swizzle both reads are free of bank conflicts (even and odd g differ in bit 2 of the row, even
+// rows of the c's are all different).  A code becomes fp16 exactly: 0x6400 | (code + 128) is 1152 + code.
 //   Online softmax per warp: the running maximum m moves only when some score exceeds it by more than kSlack in the
-// exponent (one vote per 16 tokens instead of a reduction); p = 2^(s - m + kLift) then stays below 2^15, inside fp16,
-// and a weight of 2^-21 of the largest is still a normal number.  Scores,
-// maxima, sums and accumulators are fp32; p is rounded to fp16 for the second product (relative 2^-11, against fp16
-// outputs with the same step).  With fp32 inputs or outputs (SPLIT) q and p go in as two fp16 terms each, 22 bits.
+// exponent (one vote per 16 tokens instead of a reduction); p = 2^(s - m + kLift) stays below 2^15, inside fp16, and a
+// weight of 2^-19 of the largest is still a normal number.  Scores, maxima, sums and accumulators are fp32; p is rounded to
+// fp16 for the second product (relative 2^-11, against fp16 outputs with the same step).  With fp32 inputs or outputs
+// (SPLIT) q and p go in as two fp16 terms each, 22 bits.
 //   A tile of 16 tokens lies in one block (block sizes are multiples of 16), so its scales are two scalars: sk goes into
-// the score's factor, sv multiplies the tile's own product before it is added up.
+// the score's factor, sv over a running power of two into p.
 //
-// Work: an item is (sequence, tile of rows, kv head); its keys are cut into steps of 64 tokens (16 per warp).  The steps
-// of all items in order are dealt to the CTAs in equal contiguous ranges, whatever the lengths, so a long sequence is
-// split and short ones are packed.  A CTA that holds part of an item leaves {max, sum, rows} in the workspace (at most
-// two parts per CTA) and attn_join_kernel adds the parts in order.
+// Work: an item is (sequence, tile of rows, kv head).  The steps of all items in order are dealt to the CTAs in equal
+// contiguous ranges, whatever the lengths, so a long sequence is split and short ones are packed.  A CTA that holds part of
+// an item leaves {max, sum, rows} in the workspace (at most two parts per CTA) and attn_join_kernel adds the parts in
+// order.
 #pragma once
 
-#include "ztq_common.cuh"
+#include "tc_common.cuh"
 
 namespace ztq {
 
 constexpr int kAttnMaxSeqs = 4096;
-constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
+constexpr int kAttnWarps = 8, kAttnThreads = 32 * kAttnWarps + 32;      // and the producer
 constexpr int kAttnStep = 16 * kAttnWarps;
-constexpr int kAttnMinSteps = 2;                    // steps a CTA gets at least
+constexpr int kAttnMinSteps = 1;                    // steps a CTA gets at least
+constexpr uint32_t kAttnHidden = 0xfffe5afeu;       // in place of a K scale: 16 tokens without a block (a NaN no arithmetic makes)
 constexpr float kAttnSlack = 8.f;                   // how far a score may exceed the running maximum before that moves
-constexpr float kAttnLift = 7.f;                    // p = 2^(s - m + lift): below 2^15, and its fp16 steps end at 2^-31 of the largest
+constexpr float kAttnLift = 5.f;
+constexpr int kAttnScaleSlack = 2;                  // how far a block's V scale may exceed the running power of two: p < 2^(8 + 5 + 2)
 
 struct AttnParams {
     const void* q;
@@ -54,7 +59,7 @@ struct AttnParams {
     float* parts;                                   // [grid][2] slots of 8 NT (D + 2) floats
     int seqs, tokens, max_new, q_heads, kv_heads, group, width, shift, blocks, window;
     float scale_log2;                               // softmax scale times log2(e)
-    int x_f32, y_f32, vec;
+    int x_f32, y_f32, vec, y_wide;                  // vec, y_wide: 8-byte reads of q, 16-byte stores of y
     int min_rows, max_rows;                         // sequences with more or fewer rows per kv head belong to another kernel
 };
 
@@ -117,10 +122,16 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
-__device__ __forceinline__ uint2 ld_stream8(const void* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
 }
 
 // Where CTA i's range of `total` steps begins when `ctas` of them share it.
@@ -203,31 +214,140 @@ __device__ __forceinline__ void attn_store(const AttnParams& p, const AttnSeq& s
     else static_cast<__half*>(p.y)[at] = __float2half_rn(v);
 }
 
+__device__ __forceinline__ void attn_store8(const AttnParams& p, const AttnSeq& s, int r, int h, int d, const float (&v)[8]) {
+    const long long at = (s.first + r / p.group) * p.y_token + (long long)(h * p.group + r % p.group) * p.y_head + d;
+    if (p.y_f32) {
+        float* y = static_cast<float*>(p.y) + at;
+        if (p.y_wide) {
+            *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(y + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = v[k];
+        }
+    } else {
+        __half* y = static_cast<__half*>(p.y) + at;
+        if (p.y_wide) *reinterpret_cast<uint4*>(y) = make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]), pack_half2(v[6], v[7]));
+        else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = __float2half_rn(v[k]);
+        }
+    }
+}
+
+// Shared memory of a rows CTA: the ring, the exchange between its warps, the steps' factors and the scan.
+template <int D, int NT>
+struct AttnRing {
+    static constexpr int kStepBytes = 2 * kAttnStep * D;                       // K then V
+    static constexpr int kStages = D == 64 ? 8 : D == 128 ? (NT == 1 ? 5 : 4) : 2;
+    static constexpr int kSwapBytes = kAttnWarps / 2 * 32 * (NT * D / 16 * 4 + 4 * NT) * 4;
+    static constexpr int kInfo = kStages * kAttnStep / 16;                     // {sk, sv} of every 16 tokens
+    static constexpr int kSwapAt = kStages * kStepBytes, kInfoAt = kSwapAt + kSwapBytes, kBarAt = kInfoAt + kInfo * 8, kScanAt = kBarAt + 2 * kStages * 8 + 16;
+    static constexpr int bytes(int seqs) { return kScanAt + seqs * 8 + 1024; }  // 1024: the ring starts on the swizzle's period
+};
+
 template <int D, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 && !SPLIT ? 4 : NT <= 2 && D <= 128 ? 2 : 1)
-    attn_rows_kernel(const AttnParams p) {
-    constexpr int TILE = 8 * NT, KS = D / 16, KL = D / 64;      // rows of an item, k-steps, 16-byte loads per row of K
+__global__ void __launch_bounds__(kAttnThreads, 1) attn_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttnParams p) {
+    using Ring = AttnRing<D, NT>;
+    constexpr int TILE = 8 * NT, KS = D / 16, KL = D / 64;      // rows of an item, k-steps, 16-byte pieces of a row of K per lane
     constexpr int VB = D / 8;                                   // dims of V per lane
-    extern __shared__ __align__(16) uint8_t smem[];
-    float* red = reinterpret_cast<float*>(smem);                // [warps][TILE][D + 4]: acc, then max and sum
-    long long* upto = reinterpret_cast<long long*>(smem + kAttnWarps * TILE * (D + 4) * 4);
-    __shared__ long long part[kAttnWarps];
+    constexpr int ROW = D < 128 ? D : 128;                      // bytes of a row in a swizzled tile
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    float* swap = reinterpret_cast<float*>(smem + Ring::kSwapAt);
+    float2* info = reinterpret_cast<float2*>(smem + Ring::kInfoAt);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + Ring::kBarAt);
+    uint64_t* empty = full + Ring::kStages;
+    long long* upto = reinterpret_cast<long long*>(smem + Ring::kScanAt);
+    __shared__ long long part[kAttnWarps + 1];
+    __shared__ int failed;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
 
-    grid_dep_launch();
+    if (tid == 0) {
+        for (int i = 0; i < Ring::kStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kAttnWarps);
+        }
+        failed = 0;
+        mbar_fence_init();
+    }
     grid_dep_wait();
+    grid_dep_launch();                                          // behind the wait: the join reads the lengths before its own
     attn_scan(p, TILE, upto, part);
     const long long total = upto[p.seqs - 1];
     const int ctas = attn_ctas(total, gridDim.x);
     if ((int)blockIdx.x >= ctas) return;
-    const long long w_end = attn_cut(total, blockIdx.x + 1, ctas);
+    const long long w0 = attn_cut(total, blockIdx.x, ctas), w_end = attn_cut(total, blockIdx.x + 1, ctas);
 
-    for (long long w = attn_cut(total, blockIdx.x, ctas); w < w_end;) {
+    if (warp == kAttnWarps) {
+        // ------------------------------------------------ producer: lane j < 8 looks after tokens 16 j .. of every step
+        const int per = 1 << (p.shift - 4);                     // 16-token groups of a block: the first of them in a step copies
+        int n = 0;                                              // steps issued
+        for (long long w = w0; w < w_end;) {
+            AttnSeq s;
+            const AttnItem it = attn_find(p, TILE, upto, w, s);
+            const int step0 = (int)(w - it.begin), step1 = (int)min((long long)it.steps, step0 + (w_end - w));
+            const int* table = p.block_table + (long long)it.b * p.width;
+            auto look = [&](int step) {                         // the block of this lane's group, -1 where there is none
+                const int tok = (it.lo / kAttnStep + step) * kAttnStep + 16 * (lane & 7);
+                int blk = -1;
+                if (step < step1 && tok < it.hi) {
+                    blk = table[tok >> p.shift];
+                    if ((unsigned)blk >= (unsigned)p.blocks) {
+                        report_error(ZTQ_ERR_BLOCK);
+                        blk = -1;
+                    }
+                }
+                return blk;
+            };
+            auto scales = [&](int blk) {
+                const long long at = (long long)max(blk, 0) * p.kv_heads + it.h;
+                return blk < 0 ? make_float2(__uint_as_float(kAttnHidden), 0.f) : make_float2(p.ks[at], p.vs[at]);
+            };
+            int blk = look(step0), blk1 = look(step0 + 1);
+            float2 f = scales(blk);
+            for (int step = step0; step < step1; ++step, ++n) {
+                const int blk2 = look(step + 2);
+                const float2 f1 = scales(blk1);
+                const int stage = n % Ring::kStages;
+                if (n >= Ring::kStages && !mbar_wait(&empty[stage], ((n / Ring::kStages) - 1) & 1)) {
+                    report_error(ZTQ_ERR_EMPTY_WAIT);
+                    return;
+                }
+                if (lane < 8) info[stage * 8 + lane] = f;
+                const bool copies = lane < 8 && blk >= 0 && (lane & (per - 1)) == 0;
+                const unsigned who = __ballot_sync(0xffffffffu, copies);
+                __syncwarp();                                   // the factors are written before lane 0 arrives
+                if (lane == 0) mbar_expect_tx(&full[stage], __popc(who) * 2 * ((16 * D) << (p.shift - 4)));
+                __syncwarp();
+                if (copies) {
+                    uint8_t* dst = smem + stage * Ring::kStepBytes + 16 * lane * ROW;
+                    const int row = it.h << p.shift;
+#pragma unroll
+                    for (int x = 0; x < D; x += 128) {
+                        tma_load_3d(dst + x * kAttnStep, &k_map, x, row, blk, &full[stage]);
+                        tma_load_3d(dst + kAttnStep * D + x * kAttnStep, &v_map, x, row, blk, &full[stage]);
+                    }
+                }
+                blk = blk1; blk1 = blk2; f = f1;
+            }
+            w += step1 - step0;
+        }
+        return;
+    }
+
+    // ------------------------------------------------ the other warps
+    // tau(g); tokens of the lane's V rows; byte offsets of its pieces inside its 16 tokens of a step
+    const int tau = (g & 1) ? (g + 4) & 7 : g, tv0 = 2 * c, tv1 = (2 * c + 5) & 7;
+    auto piece = [](int row, int chunk) {                       // 16-byte piece `chunk` of a row, as the copies swizzle it
+        return D == 64 ? row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4) : (chunk >> 3) * (kAttnStep * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+    };
+    int n = 0;
+    for (long long w = w0; w < w_end;) {
         AttnSeq s;
         const AttnItem it = attn_find(p, TILE, upto, w, s);
         const int step0 = (int)(w - it.begin), step1 = (int)min((long long)it.steps, step0 + (w_end - w));
-        const int rows = it.r1 - it.r0, base = s.len - s.fresh;
-        const int head = it.h * p.group;
+        const int base = s.len - s.fresh, head = it.h * p.group;
 
         // the item's queries as B fragments; columns are the rows r0 + 8 t + g
         uint32_t qh[NT][KS][2], ql[SPLIT ? NT : 1][KS][2];
@@ -240,124 +360,104 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 && !SPLIT ? 
             for (int j = 0; j < KS; ++j) {
                 const long long d0 = at + 64 * (j / 4) + 16 * c + 4 * (j % 4);
                 float v[4] = {0.f, 0.f, 0.f, 0.f};
+                uint2 u = make_uint2(0, 0);
                 if (live) {
                     if (p.x_f32) {
                         const float* f = static_cast<const float*>(p.q) + d0;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) v[i] = f[i];
                     } else if (p.vec) {
-                        const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __half*>(p.q) + d0);
-                        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-                        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+                        u = *reinterpret_cast<const uint2*>(static_cast<const __half*>(p.q) + d0);
                     } else {
-                        const __half* f = static_cast<const __half*>(p.q) + d0;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = __half2float(f[i]);
+                        const unsigned short* f = static_cast<const unsigned short*>(p.q) + d0;
+                        u = make_uint2(f[0] | (uint32_t)f[1] << 16, f[2] | (uint32_t)f[3] << 16);
                     }
                 }
-                qh[t][j][0] = pack_half2(v[0], v[1]);
-                qh[t][j][1] = pack_half2(v[2], v[3]);
                 if constexpr (SPLIT) {
-                    ql[t][j][0] = pack_rest(v[0], v[1], qh[t][j][0]);
-                    ql[t][j][1] = pack_rest(v[2], v[3], qh[t][j][1]);
+                    if (p.x_f32) u = make_uint2(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]));
+                    ql[t][j][0] = p.x_f32 ? pack_rest(v[0], v[1], u.x) : 0u;
+                    ql[t][j][1] = p.x_f32 ? pack_rest(v[2], v[3], u.y) : 0u;
                 }
+                qh[t][j][0] = u.x;
+                qh[t][j][1] = u.y;
             }
         }
 
         float acc[NT][KS][4];                                   // [dims 2 mt (+1) of the lane's][rows 2c, 2c + 1]
         float m[NT][2], l[NT][2];
+        int last[NT][2], z_min = 0x7fffffff, z_max = -1;        // last key that each of the lane's rows sees (its first is that less the window)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             m[t][0] = m[t][1] = -INFINITY;
             l[t][0] = l[t][1] = 0.f;
 #pragma unroll
             for (int j = 0; j < KS; ++j) acc[t][j][0] = acc[t][j][1] = acc[t][j][2] = acc[t][j][3] = 0.f;
-        }
-        // last key that each of the lane's rows sees (its first is that less the window)
-        int last[NT][2];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = it.r0 + 8 * t + 2 * c + i;
                 last[t][i] = r < it.r1 ? min(base + r / p.group, s.len - 1) : -1;
+                if (r < it.r1) { z_min = min(z_min, last[t][i]); z_max = max(z_max, last[t][i]); }
             }
+        }
+        z_min = __reduce_min_sync(0xffffffffu, z_min);
+        z_max = __reduce_max_sync(0xffffffffu, z_max);
+        int vrun = -1000;
 
-        const int tok0 = (it.lo / kAttnStep + step0) * kAttnStep + 16 * warp, tok1 = min(it.hi, (it.lo / kAttnStep + step1) * kAttnStep);
-        const int* table = p.block_table + (long long)it.b * p.width;
-        auto block_of = [&](int tok) {
-            int blk = table[tok >> p.shift];
-            if ((unsigned)blk >= (unsigned)p.blocks) {
-                report_error(ZTQ_ERR_BLOCK);
-                blk = -1;
+        for (int step = step0; step < step1; ++step, ++n) {
+            const int stage = n % Ring::kStages, tok = (it.lo / kAttnStep + step) * kAttnStep + 16 * warp;
+            bool came = !*(volatile int*)&failed;
+            if (came && !mbar_wait(&full[stage], (n / Ring::kStages) & 1)) {
+                report_error(ZTQ_ERR_FULL_WAIT);
+                *(volatile int*)&failed = 1;
+                came = false;
             }
-            return blk;
-        };
-        const int mask = (1 << p.shift) - 1;
-        uint4 kbuf[2][KL];
-        uint32_t vbuf[4][VB / 4];
-        int blk = tok0 < tok1 ? block_of(tok0) : -1;
-        auto load_k = [&](int blk, int tok) {
-            const int8_t* src = p.kc + max(blk, 0) * p.block_stride + (((long long)it.h << p.shift) + (tok & mask) + g) * D + 16 * c;
+            came = __all_sync(0xffffffffu, came);
+            if (tok >= it.hi || !came) {                        // nothing for this warp
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[stage]);
+                continue;
+            }
+            const uint8_t* sk = smem + stage * Ring::kStepBytes + 16 * warp * ROW;
+            const uint8_t* sv = sk + kAttnStep * D;
+            const float2 f2 = info[stage * 8 + warp];
+            const bool hidden = __float_as_uint(f2.x) == kAttnHidden;
+            // ---- scores of 16 tokens, two chains
+            float sc[NT][4], sd[NT][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int j = 0; j < KL; ++j) kbuf[i][j] = ld_stream(src + 8 * i * D + 64 * j);
-        };
-        auto load_v = [&](int blk, int tok) {
-            const int8_t* src = p.vc + max(blk, 0) * p.block_stride + (((long long)it.h << p.shift) + (tok & mask) + 2 * c) * D + VB * g;
+                for (int i = 0; i < 4; ++i) sc[t][i] = sd[t][i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int8_t* row = src + ((i & 1) + 8 * (i >> 1)) * D;
-                if constexpr (VB == 8) {
-                    const uint2 u = ld_stream8(row);
-                    vbuf[i][0] = u.x; vbuf[i][1] = u.y;
-                } else {
+            for (int l4 = 0; l4 < KL; ++l4) {
+                const uint4 a4 = *reinterpret_cast<const uint4*>(sk + piece(tau, c + 4 * l4)), b4 = *reinterpret_cast<const uint4*>(sk + piece(tau + 8, c + 4 * l4));
+                const uint32_t xs[4] = {a4.x, a4.y, a4.z, a4.w}, ys[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-                    for (int j = 0; j < VB / 16; ++j) {
-                        const uint4 u = ld_stream(row + 16 * j);
-                        vbuf[i][4 * j] = u.x; vbuf[i][4 * j + 1] = u.y; vbuf[i][4 * j + 2] = u.z; vbuf[i][4 * j + 3] = u.w;
+                for (int k = 0; k < 4; ++k) {
+                    const int j = 4 * l4 + k;
+                    const uint32_t x = xs[k] ^ 0x80808080u, y = ys[k] ^ 0x80808080u;
+                    const uint32_t a[4] = {unbias(__byte_perm(x, 0x64646464u, 0x4140)), unbias(__byte_perm(y, 0x64646464u, 0x4140)),
+                                           unbias(__byte_perm(x, 0x64646464u, 0x4342)), unbias(__byte_perm(y, 0x64646464u, 0x4342))};
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        mma_f16(j & 1 ? sd[t] : sc[t], a, qh[t][j][0], qh[t][j][1]);
+                        if constexpr (SPLIT) mma_f16(j & 1 ? sc[t] : sd[t], a, ql[t][j][0], ql[t][j][1]);
                     }
                 }
             }
-        };
-        if (tok0 < tok1) {
-            load_k(blk, tok0);
-            load_v(blk, tok0);
-        }
-        for (int tok = tok0; tok < tok1; tok += kAttnStep) {
-            const int next = tok + kAttnStep;
-            const int blk_next = next < tok1 ? block_of(next) : -1;
-            const float ks = blk >= 0 ? p.ks[(long long)blk * p.kv_heads + it.h] : 0.f;
-            float vs = blk >= 0 ? p.vs[(long long)blk * p.kv_heads + it.h] : 0.f;
-            // ---- scores of 16 tokens
-            float sc[NT][4];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
-#pragma unroll
-            for (int j = 0; j < KS; ++j) {
-                const uint4 w0 = kbuf[0][j / 4], w1 = kbuf[1][j / 4];
-                const uint32_t x = (j % 4 == 0 ? w0.x : j % 4 == 1 ? w0.y : j % 4 == 2 ? w0.z : w0.w) ^ 0x80808080u;
-                const uint32_t y = (j % 4 == 0 ? w1.x : j % 4 == 1 ? w1.y : j % 4 == 2 ? w1.z : w1.w) ^ 0x80808080u;
-                const uint32_t a[4] = {unbias(__byte_perm(x, 0x64646464u, 0x4140)), unbias(__byte_perm(y, 0x64646464u, 0x4140)),
-                                       unbias(__byte_perm(x, 0x64646464u, 0x4342)), unbias(__byte_perm(y, 0x64646464u, 0x4342))};
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    mma_f16(sc[t], a, qh[t][j][0], qh[t][j][1]);
-                    if constexpr (SPLIT) mma_f16(sc[t], a, ql[t][j][0], ql[t][j][1]);
-                }
-            }
-            if (next < tok1) load_k(blk_next, next);
             // ---- masks and the running maximum
-            const float f = ks * p.scale_log2;
+            const float f = f2.x * p.scale_log2;
+            const bool whole_tile = !hidden && tok + 15 <= z_min && (p.window <= 0 || tok > z_max - p.window);
             bool grows = false;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int key = tok + g + 8 * (i >> 1), z = last[t][i & 1];
-                    const bool seen = blk >= 0 && key <= z && (p.window <= 0 || key > z - p.window);
-                    sc[t][i] = seen ? sc[t][i] * f : -INFINITY;
+                    sc[t][i] = (sc[t][i] + sd[t][i]) * f;
+                    if (!whole_tile) {
+                        const int key = tok + tau + 8 * (i >> 1), z = last[t][i & 1];
+                        const bool seen = !hidden && key <= z && (p.window <= 0 || key > z - p.window);
+                        sc[t][i] = seen ? sc[t][i] : -INFINITY;
+                    }
                     grows |= sc[t][i] > m[t][i & 1] + kAttnSlack;
                 }
             if (__any_sync(0xffffffffu, grows)) {
@@ -369,7 +469,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 && !SPLIT ? 
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                         if (top > m[t][i]) {
-                            const float fix = m[t][i] == -INFINITY ? 0.f : exp2f(m[t][i] - top);
+                            const float fix = m[t][i] == -INFINITY ? 0.f : ex2(m[t][i] - top);
                             l[t][i] *= fix;
 #pragma unroll
                             for (int j = 0; j < KS; ++j) { acc[t][j][i] *= fix; acc[t][j][i + 2] *= fix; }
@@ -377,15 +477,42 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 && !SPLIT ? 
                         }
                     }
             }
+            // ---- the V scale over the running power of two
+            float r = 0.f;
+            if (fabsf(f2.y) <= 3.402823466e38f) {
+                const int e = min(max((int)(__float_as_uint(fabsf(f2.y)) >> 23) - 127, -120), 120);
+                if (e > vrun + kAttnScaleSlack) {
+                    const float fix = vrun > -1000 ? ex2((float)max(vrun - e, -126)) : 0.f;
+                    vrun = e;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int j = 0; j < KS; ++j)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[t][j][i] *= fix;
+                }
+                r = f2.y * __uint_as_float((uint32_t)(127 - vrun) << 23);
+            } else {                                            // NaN for the rows that see the tile, not for the masked ones
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        unsigned sees = __ballot_sync(0xffffffffu, sc[t][i] != -INFINITY || sc[t][i + 2] != -INFINITY);
+                        sees |= sees >> 16; sees |= sees >> 8; sees |= sees >> 4;
+                        if (sees >> c & 1) l[t][i] = __int_as_float(0x7fc00000);
+                    }
+            }
             // ---- p as B fragments
             uint32_t ph[NT][2], pl[SPLIT ? NT : 1][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
+                const float shift0 = kAttnLift - (m[t][0] == -INFINITY ? 0.f : m[t][0]), shift1 = kAttnLift - (m[t][1] == -INFINITY ? 0.f : m[t][1]);
                 float e[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    e[i] = sc[t][i] == -INFINITY ? 0.f : exp2f(sc[t][i] - m[t][i & 1] + kAttnLift);
+                    e[i] = ex2(sc[t][i] + (i & 1 ? shift1 : shift0));
                     l[t][i & 1] += e[i];
+                    e[i] *= r;
                 }
                 const uint32_t h0 = pack_half2(e[0], e[1]), h1 = pack_half2(e[2], e[3]);
                 ph[t][0] = transpose8x8(h0);
@@ -396,151 +523,193 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 && !SPLIT ? 
                 }
             }
             // ---- their values: four dims of four tokens at a time
-            if (!(fabsf(vs) <= 3.402823466e38f)) {              // reaches the rows that see the tile, not the masked ones
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+            for (int v4 = 0; v4 < (VB + 15) / 16; ++v4) {
+                uint32_t vb[4][VB < 16 ? 2 : 4];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const bool sees = sc[t][i] != -INFINITY || sc[t][i + 2] != -INFINITY;
-                        unsigned who = __ballot_sync(0xffffffffu, sees);
-                        who |= who >> 16; who |= who >> 8; who |= who >> 4;
-                        if (who >> c & 1) l[t][i] = __int_as_float(0x7fc00000);
+                for (int i = 0; i < 4; ++i) {
+                    const int row = (i & 1 ? tv1 : tv0) + 8 * (i >> 1);
+                    if constexpr (VB < 16) {
+                        const uint2 u = *reinterpret_cast<const uint2*>(sv + piece(row, g >> 1) + 8 * (g & 1));
+                        vb[i][0] = u.x; vb[i][1] = u.y;
+                    } else {
+                        const uint4 u = *reinterpret_cast<const uint4*>(sv + piece(row, g + 8 * v4));
+                        vb[i][0] = u.x; vb[i][1] = u.y; vb[i][2] = u.z; vb[i][3] = u.w;
                     }
-                vs = 0.f;
-            }
+                }
 #pragma unroll
-            for (int q4 = 0; q4 < VB / 4; ++q4) {
-                const uint32_t x0 = vbuf[0][q4] ^ 0x80808080u, x1 = vbuf[1][q4] ^ 0x80808080u, x2 = vbuf[2][q4] ^ 0x80808080u, x3 = vbuf[3][q4] ^ 0x80808080u;
-                const uint32_t lo01 = __byte_perm(x0, x1, 0x5140), hi01 = __byte_perm(x0, x1, 0x7362);     // dims 0, 1 | 2, 3 of both
-                const uint32_t lo23 = __byte_perm(x2, x3, 0x5140), hi23 = __byte_perm(x2, x3, 0x7362);
+                for (int q4 = 0; q4 < (VB < 16 ? 2 : 4); ++q4) {
+                    const uint32_t x0 = vb[0][q4] ^ 0x80808080u, x1 = vb[1][q4] ^ 0x80808080u, x2 = vb[2][q4] ^ 0x80808080u, x3 = vb[3][q4] ^ 0x80808080u;
+                    const uint32_t lo01 = __byte_perm(x0, x1, 0x5140), hi01 = __byte_perm(x0, x1, 0x7362);     // dims 0, 1 | 2, 3 of both
+                    const uint32_t lo23 = __byte_perm(x2, x3, 0x5140), hi23 = __byte_perm(x2, x3, 0x7362);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint32_t u = half ? hi01 : lo01, v = half ? hi23 : lo23;
-                    const uint32_t a[4] = {unbias(__byte_perm(u, 0x64646464u, 0x4140)), unbias(__byte_perm(u, 0x64646464u, 0x4342)),
-                                           unbias(__byte_perm(v, 0x64646464u, 0x4140)), unbias(__byte_perm(v, 0x64646464u, 0x4342))};
-                    const int mt = 2 * q4 + half;
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t u = half ? hi01 : lo01, v = half ? hi23 : lo23;
+                        const uint32_t a[4] = {unbias(__byte_perm(u, 0x64646464u, 0x4140)), unbias(__byte_perm(u, 0x64646464u, 0x4342)),
+                                               unbias(__byte_perm(v, 0x64646464u, 0x4140)), unbias(__byte_perm(v, 0x64646464u, 0x4342))};
+                        const int mt = 8 * v4 + 2 * q4 + half;
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        float o[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_f16(o, a, ph[t][0], ph[t][1]);
-                        if constexpr (SPLIT) mma_f16(o, a, pl[t][0], pl[t][1]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[t][mt][i] = fmaf(vs, o[i], acc[t][mt][i]);
+                        for (int t = 0; t < NT; ++t) {
+                            mma_f16(acc[t][mt], a, ph[t][0], ph[t][1]);
+                            if constexpr (SPLIT) mma_f16(acc[t][mt], a, pl[t][0], pl[t][1]);
+                        }
                     }
                 }
             }
-            if (next < tok1) load_v(blk_next, next);
-            blk = blk_next;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[stage]);
         }
 
-        // ---- the warps' parts meet in shared memory
-        __syncthreads();                                        // the previous segment's readers are done
+        // ---- the warps' parts meet: 8 -> 4 -> 2 -> 1, in a fixed order
+        {
+            const float vref = vrun > -1000 ? ex2((float)vrun) : 0.f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float sum = l[t][i];
+                for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                float* row = red + (warp * TILE + 8 * t + 2 * c + i) * (D + 4);
+                    for (int o = 4; o < 32; o <<= 1) l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], o);
 #pragma unroll
-                for (int j = 0; j < KS; ++j) {
-                    row[VB * g + 2 * j] = acc[t][j][i];
-                    row[VB * g + 2 * j + 1] = acc[t][j][i + 2];
+                    for (int j = 0; j < KS; ++j) { acc[t][j][i] *= vref; acc[t][j][i + 2] *= vref; }
                 }
-                if (g == 0) { row[D] = m[t][i]; row[D + 1] = sum; }
-            }
-        __syncthreads();
-        const bool whole = step0 == 0 && step1 == it.steps;
-        float* out = p.parts + ((long long)blockIdx.x * 2 + (step0 == 0 ? 1 : 0)) * TILE * (D + 2);
-        for (int i = tid; i < rows * D; i += kAttnThreads) {
-            const int r = i / D, d = i % D;
-            float top = -INFINITY;
+        }
 #pragma unroll
-            for (int u = 0; u < kAttnWarps; ++u) top = fmaxf(top, red[(u * TILE + r) * (D + 4) + D]);
-            float sum = 0.f, v = 0.f;
+        for (int half = kAttnWarps / 2; half > 0; half >>= 1) {
+            bar_sync(1, 32 * kAttnWarps);                       // what the exchange held before has been read
+            float4* mine = reinterpret_cast<float4*>(swap) + (warp % half) * 32 * (NT * KS + NT) + lane;
+            if (warp >= half && warp < 2 * half) {
 #pragma unroll
-            for (int u = 0; u < kAttnWarps; ++u) {
-                const float* row = red + (u * TILE + r) * (D + 4);
-                const float fix = row[D] == -INFINITY ? 0.f : exp2f(row[D] - top);
-                sum += fix * row[D + 1];
-                v += fix * row[d];
+                for (int t = 0; t < NT; ++t) {
+                    mine[32 * (NT * KS + t)] = make_float4(m[t][0], m[t][1], l[t][0], l[t][1]);
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) mine[32 * (t * KS + j)] = make_float4(acc[t][j][0], acc[t][j][1], acc[t][j][2], acc[t][j][3]);
+                }
             }
-            if (whole) attn_store(p, s, it.r0 + r, it.h, d, sum > 0.f || sum != sum ? v / sum : 0.f);
-            else {
-                out[r * (D + 2) + d] = v;
-                if (d == 0) { out[r * (D + 2) + D] = top; out[r * (D + 2) + D + 1] = sum; }
+            bar_sync(1, 32 * kAttnWarps);
+            if (warp < half) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const float4 o = mine[32 * (NT * KS + t)];
+                    float f0[2], f1[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float mo = i ? o.y : o.x, lo = i ? o.w : o.z, top = fmaxf(m[t][i], mo);
+                        f0[i] = m[t][i] == -INFINITY ? 0.f : ex2(m[t][i] - top);
+                        f1[i] = mo == -INFINITY ? 0.f : ex2(mo - top);
+                        l[t][i] = f0[i] * l[t][i] + f1[i] * lo;
+                        m[t][i] = top;
+                    }
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) {
+                        const float4 x = mine[32 * (t * KS + j)];
+                        acc[t][j][0] = f0[0] * acc[t][j][0] + f1[0] * x.x;
+                        acc[t][j][1] = f0[1] * acc[t][j][1] + f1[1] * x.y;
+                        acc[t][j][2] = f0[0] * acc[t][j][2] + f1[0] * x.z;
+                        acc[t][j][3] = f0[1] * acc[t][j][3] + f1[1] * x.w;
+                    }
+                }
             }
+        }
+        if (warp == 0 && !*(volatile int*)&failed) {
+            const bool whole = step0 == 0 && step1 == it.steps;
+            float* out = p.parts + ((long long)blockIdx.x * 2 + (step0 == 0 ? 1 : 0)) * TILE * (D + 2);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = 8 * t + 2 * c + i;
+                    if (it.r0 + r >= it.r1) continue;
+                    const float inv = whole ? (l[t][i] > 0.f || l[t][i] != l[t][i] ? 1.f / l[t][i] : 0.f) : 1.f;
+#pragma unroll
+                    for (int j = 0; j < KS; j += 4) {           // eight consecutive dims of the lane's
+                        const int d = VB < 16 ? VB * g : 128 * (j / 8) + 16 * g + 2 * (j % 8);
+                        float v[8];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) { v[2 * k] = acc[t][j + k][i] * inv; v[2 * k + 1] = acc[t][j + k][i + 2] * inv; }
+                        if (whole) attn_store8(p, s, it.r0 + r, it.h, d, v);
+                        else {
+#pragma unroll
+                            for (int k = 0; k < 8; k += 2) *reinterpret_cast<float2*>(out + r * (D + 2) + d + k) = make_float2(v[k], v[k + 1]);
+                        }
+                    }
+                    if (!whole && g == 0) *reinterpret_cast<float2*>(out + r * (D + 2) + D) = make_float2(m[t][i], l[t][i]);
+                }
         }
         w += step1 - step0;
     }
 }
 
-// Adds the parts of the items that several CTAs shared.  blockIdx.x = j looks at the boundary between the ranges of CTAs j
-// and j + 1 of attn_rows_kernel and does the item it cuts, if it is the first boundary inside that item; blockIdx.y is the
-// row.  A short row of long loads: the parts' maxima and sums are fetched together, then every warp adds its share of the
-// parts (all loads independent), then the warps' sums are added in order.
+// Adds the parts of the items that several CTAs shared: blockIdx.x = j looks at the boundary between the ranges of CTAs j and
+// j + 1 of attn_rows_kernel and does the item it cuts, if it is the first boundary inside that item.  `share` warps take a
+// row (all of a CTA's where items are few and have many parts): every warp adds its share of the parts, all loads
+// independent, then the warps' sums are added in order.
 constexpr int kJoinThreads = 256;
 template <int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnParams p, int grid) {
     constexpr int TILE = 8 * NT, V = D / 32, WARPS = kJoinThreads / 32;   // V: dims per lane
-    extern __shared__ __align__(16) uint8_t smem[];
-    long long* upto = reinterpret_cast<long long*>(smem);
-    float* fix = reinterpret_cast<float*>(upto + p.seqs);                  // [parts], at most one per CTA
+    extern __shared__ __align__(16) uint8_t smem_join[];
+    long long* upto = reinterpret_cast<long long*>(smem_join);
     __shared__ long long part[WARPS];
-    __shared__ float red[WARPS][D + 1];
+    __shared__ float red[WARPS][D + 2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     grid_dep_launch();
-    grid_dep_wait();
-    attn_scan(p, TILE, upto, part);
+    attn_scan(p, TILE, upto, part);                        // the lengths are older than the kernel in front (see there)
     const long long total = upto[p.seqs - 1];
-    const int ctas = attn_ctas(total, grid), cta = blockIdx.x, r = blockIdx.y;
-    if (cta + 1 >= ctas) return;
-    const long long w = attn_cut(total, cta + 1, ctas);
-    AttnSeq s;
-    const AttnItem it = attn_find(p, TILE, upto, w, s);
-    if (it.begin == w || attn_cut(total, cta, ctas) > it.begin || r >= it.r1 - it.r0) return;     // no cut inside, or not the first one
+    const int ctas = attn_ctas(total, grid), cta = blockIdx.x, share = WARPS * gridDim.y / TILE;     // warps per row: 1 or WARPS
+    const bool cuts = cta + 1 < ctas;
+    const long long w = cuts ? attn_cut(total, cta + 1, ctas) : 0;
+    AttnSeq s = {};
+    AttnItem it = {};
+    if (cuts) it = attn_find(p, TILE, upto, w, s);
+    // Every CTA waits, also one with nothing to do: the kernel behind this one takes its end for the end of the one in front.
+    grid_dep_wait();
+    if (!cuts || it.begin == w || attn_cut(total, cta, ctas) > it.begin) return;     // no cut inside, or not the first one
     // CTAs cta .. cta + n - 1 hold parts; the last is the one whose range reaches the item's end
     const long long end = it.begin + it.steps;
     int last = (int)(end * ctas / total);
     while (last > cta && attn_cut(total, last, ctas) >= end) --last;
     while (attn_cut(total, last + 1, ctas) < end) ++last;
-    const int n = last - cta + 1;
-    auto row_of = [&](int u) { return p.parts + ((long long)(cta + u) * 2 + (u == 0 ? 1 : 0)) * TILE * (D + 2) + r * (D + 2); };
-    float top = -INFINITY;
-    for (int u = tid; u < n; u += kJoinThreads) {
-        const float m = row_of(u)[D];
-        fix[u] = m;
-        top = fmaxf(top, m);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) red[warp][0] = top;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < WARPS; ++k) top = fmaxf(top, red[k][0]);
-    __syncthreads();
-    float sum = 0.f, v[V];
+    const int n = last - cta + 1, r = share == 1 ? blockIdx.y * WARPS + warp : blockIdx.y;
+    float top = -INFINITY, sum = 0.f, v[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = 0.f;
+    if (r < it.r1 - it.r0) {
 #pragma unroll 4
-    for (int u = warp; u < n; u += WARPS) {
-        const float* row = row_of(u);
-        const float f = fix[u] == -INFINITY ? 0.f : exp2f(fix[u] - top);
-        sum += f * row[D + 1];
+        for (int u = share == 1 ? 0 : warp; u < n; u += share) {
+            const float* row = p.parts + ((long long)(cta + u) * 2 + (u == 0 ? 1 : 0)) * TILE * (D + 2) + r * (D + 2);
+            const float2 ml = *reinterpret_cast<const float2*>(row + D);
+            float x[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] += f * row[32 * k + lane];
+            for (int k = 0; k < V; ++k) x[k] = row[32 * k + lane];
+            const float up = fmaxf(top, ml.x), old = top == -INFINITY ? 0.f : ex2(top - up), fix = ml.x == -INFINITY ? 0.f : ex2(ml.x - up);
+            sum = old * sum + fix * ml.y;
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] = old * v[k] + fix * x[k];
+            top = up;
+        }
     }
+    if (share > 1) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) red[warp][32 * k + lane] = v[k];
-    if (lane == 0) red[warp][D] = sum;
-    __syncthreads();
-    for (int d = tid; d < D; d += kJoinThreads) {
-        float a = 0.f, b = 0.f;
+        for (int k = 0; k < V; ++k) red[warp][32 * k + lane] = v[k];
+        if (lane == 0) { red[warp][D] = top; red[warp][D + 1] = sum; }
+        __syncthreads();
+        if (warp) return;
+        sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < WARPS; ++k) { a += red[k][d]; b += red[k][D]; }
-        attn_store(p, s, it.r0 + r, it.h, d, b > 0.f || b != b ? a / b : 0.f);
+        for (int k = 0; k < V; ++k) v[k] = 0.f;
+#pragma unroll
+        for (int u = 0; u < WARPS; ++u) top = fmaxf(top, red[u][D]);
+#pragma unroll
+        for (int u = 0; u < WARPS; ++u) {
+            const float fix = red[u][D] == -INFINITY ? 0.f : ex2(red[u][D] - top);
+            sum += fix * red[u][D + 1];
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] += fix * red[u][32 * k + lane];
+        }
     }
+    if (r >= it.r1 - it.r0) return;
+#pragma unroll
+    for (int k = 0; k < V; ++k) attn_store(p, s, it.r0 + r, it.h, 32 * k + lane, sum > 0.f || sum != sum ? v[k] / sum : 0.f);
 }
 
 }  // namespace ztq

@@ -106,11 +106,6 @@ __device__ __forceinline__ bool tca_item(const AttnParams& p, const int* upto, l
     return true;
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32]) {
     uint32_t r[32];
     asm volatile(
@@ -454,7 +449,6 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
         const float inv = l > 0.f || l != l ? vref / l : 0.f;
         float* part = tp.parts + (((long long)blockIdx.x * tp.splits + blockIdx.y) * kTcaRows + (r - it.r0)) * (D + 2);
         const long long to = live ? (it.s.first + r / p.group) * p.y_token + (long long)(it.h * p.group + r % p.group) * p.y_head : 0;
-        const bool wide = p.y_token % 8 == 0 && p.y_head % 8 == 0 && ((uintptr_t)p.y & 15) == 0;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
             float o[32];
@@ -469,7 +463,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                 for (int k = 0; k < 32; k += 2) *reinterpret_cast<float2*>(part + 32 * c + k) = make_float2(o[k] * vref, o[k + 1] * vref);
             } else {
                 __half* y = static_cast<__half*>(p.y) + to + 32 * c;
-                if (wide) {
+                if (p.y_wide) {
 #pragma unroll
                     for (int k = 0; k < 32; k += 8)
                         *reinterpret_cast<uint4*>(y + k) = make_uint4(pack_half2(o[k] * inv, o[k + 1] * inv), pack_half2(o[k + 2] * inv, o[k + 3] * inv),

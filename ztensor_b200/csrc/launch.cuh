@@ -1,6 +1,7 @@
 // launch.cuh -- host helpers shared by the translation units of libztq_sm100a.so.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 
@@ -70,6 +71,23 @@ static cudaError_t allow_smem(Kern kern, std::atomic<unsigned>& done, int bytes 
     if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
     else cudaGetLastError();                              // reported by the return value, not to the caller's next check
     return e;
+}
+
+// cuTensorMapEncodeTiled, looked up at run time (the library does not link against the driver).
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiledFn encode_tiled_fn() {
+    static std::atomic<void*> cached{nullptr};
+    void* f = cached.load(std::memory_order_acquire);
+    if (!f) {
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return nullptr;
+        cached.store(f, std::memory_order_release);
+    }
+    return reinterpret_cast<EncodeTiledFn>(f);
 }
 
 }  // namespace ztq

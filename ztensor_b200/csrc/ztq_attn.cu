@@ -11,27 +11,42 @@
 
 namespace ztq {
 
-// Rows of a tile of attn_rows_kernel and its CTAs per SM: heads of 256 leave registers for eight rows only.
-static int attn_nt(int head_dim, long long rows) { return rows <= 8 || head_dim > 128 ? 1 : 2; }
-static int attn_ctas_per_sm(int head_dim, int nt, bool split) { return nt == 1 && head_dim <= 128 && !split ? 4 : head_dim <= 128 ? 2 : 1; }
+// Row tiles of eight that a CTA of attn_rows_kernel takes at a time: two where its registers hold them.
+static int attn_nt(int head_dim, long long rows, bool split) { return rows <= 8 || head_dim > 128 || (split && head_dim > 64) ? 1 : 2; }
+
+// One layer's keys or values as (dim, head and token, block), copied a block of one head at a time.
+static bool cache_map(CUtensorMap* map, const void* base, const AttnParams& p, int dim) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)p.kv_heads << p.shift, (cuuint64_t)p.blocks}, strides[2] = {(cuuint64_t)dim, (cuuint64_t)p.block_stride};
+    const cuuint32_t box[3] = {(cuuint32_t)std::min(dim, 128), 1u << p.shift, 1}, ones[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 template <int D, int NT, bool SPLIT>
 static cudaError_t launch_rows(const AttnParams& p, int sms, cudaStream_t stream, bool pdl) {
-    const int grid = sms * attn_ctas_per_sm(D, NT, SPLIT);
+    CUtensorMap k_map, v_map;
+    if (!cache_map(&k_map, p.kc, p, D) || !cache_map(&v_map, p.vc, p, D)) return cudaErrorInvalidValue;
     static std::atomic<unsigned> done{0};
     auto kern = attn_rows_kernel<D, NT, SPLIT>;
-    if (cudaError_t e = allow_smem(kern, done, 200 * 1024)) return e;
-    const size_t upto = (size_t)p.seqs * 8;
-    cudaError_t e = launch(kern, dim3(grid), dim3(kAttnThreads), kAttnWarps * 8 * NT * (D + 4) * 4 + upto, stream, pdl, p);
-    if (e != cudaSuccess) return e;
-    e = launch(attn_join_kernel<D, NT>, dim3(grid - 1, 8 * NT), dim3(kJoinThreads), upto + grid * sizeof(float), stream, pdl, p, grid);
+    const int smem = AttnRing<D, NT>::bytes(p.seqs);
+    if (cudaError_t e = allow_smem(kern, done, AttnRing<D, NT>::bytes(kAttnMaxSeqs))) return e;
+    cudaError_t e = launch(kern, dim3(sms), dim3(kAttnThreads), smem, stream, pdl, k_map, v_map, p);
+    if (e != cudaSuccess || sms < 2) return e;
+    // many parts per row: a CTA per row; else a warp per row
+    const bool few = (long long)p.seqs * p.kv_heads <= 32;
+    e = launch(attn_join_kernel<D, NT>, dim3(sms - 1, few ? 8 * NT : NT), dim3(kJoinThreads), p.seqs * 8, stream, pdl, p, sms);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 template <int D>
 static cudaError_t launch_dim(const AttnParams& p, int nt, bool split, int sms, cudaStream_t stream, bool pdl) {
+    if constexpr (D == 64) {
+        if (nt == 2 && split) return launch_rows<D, 2, true>(p, sms, stream, pdl);
+    }
     if constexpr (D <= 128) {
-        if (nt == 2) return split ? launch_rows<D, 2, true>(p, sms, stream, pdl) : launch_rows<D, 2, false>(p, sms, stream, pdl);
+        if (nt == 2) return launch_rows<D, 2, false>(p, sms, stream, pdl);
     }
     return split ? launch_rows<D, 1, true>(p, sms, stream, pdl) : launch_rows<D, 1, false>(p, sms, stream, pdl);
 }
@@ -93,8 +108,8 @@ size_t ztq_attn_q8_workspace_bytes(int tokens, int sequences, int max_new, int q
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
     const int sms = device_info().sms > 0 ? device_info().sms : 148, group = q_heads / kv_heads;
     const long long rows = (long long)max_new * group;
-    const int nt = attn_nt(head_dim, rows);
-    return std::max((size_t)sms * attn_ctas_per_sm(head_dim, nt, false) * 2 * 8 * nt * (head_dim + 2) * sizeof(float),
+    const int nt = attn_nt(head_dim, rows, false);
+    return std::max((size_t)sms * 2 * 8 * nt * (head_dim + 2) * sizeof(float),
                     tc_plan(tokens, sequences, rows, group, kv_heads, head_dim, sms).bytes);
 }
 
@@ -143,10 +158,12 @@ cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_h
     p.x_f32 = (flags & ZTQ_X_F32) ? 1 : 0;
     p.y_f32 = (flags & ZTQ_Y_F32) ? 1 : 0;
     p.vec = ((uintptr_t)q & 7) == 0 && q_token % 4 == 0 && q_head % 4 == 0;
+    const int wide = p.y_f32 ? 4 : 8;
+    p.y_wide = ((uintptr_t)y & 15) == 0 && y_token % wide == 0 && y_head % wide == 0;
     p.min_rows = 1;
     p.max_rows = 0x7fffffff;
-    const int nt = attn_nt(dim, (long long)max_new * p.group);
     const bool split = p.x_f32 || p.y_f32, pdl = !(flags & ZTQ_NO_PDL);
+    const int nt = attn_nt(dim, (long long)max_new * p.group, split);
     if (!split) {
         const TcPlan plan = tc_plan(tokens, sequences, (long long)max_new * p.group, p.group, p.kv_heads, dim, dev.sms);
         if (plan.items > 0x7fffffff) return cudaErrorInvalidValue;

@@ -388,22 +388,6 @@ int ztq_take_error_attn();
 
 // ---- batch >= 16: W4A16 skinny GEMM on tcgen05 / TMEM -------------------------------
 namespace {
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_tiled_fn() {
-    static std::atomic<void*> cached{nullptr};
-    void* f = cached.load(std::memory_order_acquire);
-    if (!f) {
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            return nullptr;
-        cached.store(f, std::memory_order_release);
-    }
-    return reinterpret_cast<EncodeTiledFn>(f);
-}
-
 template <int NB, bool I8, bool SPLIT, int GB = 1, bool AR = false, bool W8 = false>
 cudaError_t launch_tc(const CUtensorMap& map, const TcParams& tp, int grid, size_t smem, cudaStream_t stream, bool pdl) {
     auto kern = gemm_w4g_tc_kernel<NB, I8, SPLIT, GB, AR, W8>;
