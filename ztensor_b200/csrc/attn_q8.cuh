@@ -8,7 +8,9 @@
 // together, 8 NT of them at a time, so that a block of the cache is read once for all of them.  Bound by HBM while the
 // rows of an item fit one tile (decoding, drafts).
 //   One CTA per SM: a producer warp keeps a ring of steps of 128 tokens (32 KB at D = 128) filled by tiled TMA copies, one
-// per block, and looks up block table and scales one step ahead; eight warps take 16 tokens of each step.
+// per block, and looks up block table and scales one step ahead; the other warps take 16 tokens of a step in turn.  Twelve of
+// them where 128 registers suffice: a warp's tile is a chain of 380 instructions that eight warps leave half hidden
+// (64 sequences of 3000 to 12000 tokens, 958 MB: 211 us with eight).
 //   S^T = K Q^T and Y^T = V^T P^T by mma.sync m16n8k16 with the TOKENS (then the dims) as M and the rows as N = 8: a
 // decode step has 4 to 8 rows per kv head, which as M would waste half of every instruction and more.
 //   The contraction index may be permuted as long as both operands agree, so every lane reads 16 contiguous bytes of the
@@ -36,8 +38,7 @@
 namespace ztq {
 
 constexpr int kAttnMaxSeqs = 4096;
-constexpr int kAttnWarps = 8, kAttnThreads = 32 * kAttnWarps + 32;      // and the producer
-constexpr int kAttnStep = 16 * kAttnWarps;
+constexpr int kAttnStep = 128;                      // tokens of a step: eight tiles of 16, dealt to the warps in turn
 constexpr int kAttnMinSteps = 1;                    // steps a CTA gets at least
 constexpr uint32_t kAttnHidden = 0xfffe5afeu;       // in place of a K scale: 16 tokens without a block (a NaN no arithmetic makes)
 constexpr float kAttnSlack = 8.f;                   // how far a score may exceed the running maximum before that moves
@@ -236,19 +237,22 @@ __device__ __forceinline__ void attn_store8(const AttnParams& p, const AttnSeq& 
 }
 
 // Shared memory of a rows CTA: the ring, the exchange between its warps, the steps' factors and the scan.
-template <int D, int NT>
+template <int D, int NT, bool SPLIT>
 struct AttnRing {
+    static constexpr int kWarps = NT == 1 && D <= 128 && !SPLIT ? 12 : 8;      // and the producer
+    static constexpr int kThreads = 32 * kWarps + 32;
     static constexpr int kStepBytes = 2 * kAttnStep * D;                       // K then V
     static constexpr int kStages = D == 64 ? 8 : D == 128 ? (NT == 1 ? 5 : 4) : 2;
-    static constexpr int kSwapBytes = kAttnWarps / 2 * 32 * (NT * D / 16 * 4 + 4 * NT) * 4;
+    static constexpr int kSwapBytes = kWarps / 2 * 32 * (NT * D / 16 * 4 + 4 * NT) * 4;
     static constexpr int kInfo = kStages * kAttnStep / 16;                     // {sk, sv} of every 16 tokens
     static constexpr int kSwapAt = kStages * kStepBytes, kInfoAt = kSwapAt + kSwapBytes, kBarAt = kInfoAt + kInfo * 8, kScanAt = kBarAt + 2 * kStages * 8 + 16;
     static constexpr int bytes(int seqs) { return kScanAt + seqs * 8 + 1024; }  // 1024: the ring starts on the swizzle's period
 };
 
 template <int D, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kAttnThreads, 1) attn_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttnParams p) {
-    using Ring = AttnRing<D, NT>;
+__global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const AttnParams p) {
+    using Ring = AttnRing<D, NT, SPLIT>;
+    constexpr int kAttnWarps = Ring::kWarps;
     constexpr int TILE = 8 * NT, KS = D / 16, KL = D / 64;      // rows of an item, k-steps, 16-byte pieces of a row of K per lane
     constexpr int VB = D / 8;                                   // dims of V per lane
     constexpr int ROW = D < 128 ? D : 128;                      // bytes of a row in a swizzled tile
@@ -280,7 +284,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_rows_kernel(const __grid
     const long long w0 = attn_cut(total, blockIdx.x, ctas), w_end = attn_cut(total, blockIdx.x + 1, ctas);
 
     if (warp == kAttnWarps) {
-        // ------------------------------------------------ producer: lane j < 8 looks after tokens 16 j .. of every step
+        // ------------------------------------------------ producer: lane 8 k + j looks after tokens 16 j .. of the k-th of four
+        // steps; their blocks and scales are fetched while the four before are issued (two loads that wait for one another
+        // would otherwise take as long as a step's copies: 211 -> 170 us on the case above)
         const int per = 1 << (p.shift - 4);                     // 16-token groups of a block: the first of them in a step copies
         int n = 0;                                              // steps issued
         for (long long w = w0; w < w_end;) {
@@ -288,8 +294,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_rows_kernel(const __grid
             const AttnItem it = attn_find(p, TILE, upto, w, s);
             const int step0 = (int)(w - it.begin), step1 = (int)min((long long)it.steps, step0 + (w_end - w));
             const int* table = p.block_table + (long long)it.b * p.width;
-            auto look = [&](int step) {                         // the block of this lane's group, -1 where there is none
-                const int tok = (it.lo / kAttnStep + step) * kAttnStep + 16 * (lane & 7);
+            auto look = [&](int first) {                        // the block of this lane's group, -1 where there is none
+                const int step = first + (lane >> 3), tok = (it.lo / kAttnStep + step) * kAttnStep + 16 * (lane & 7);
                 int blk = -1;
                 if (step < step1 && tok < it.hi) {
                     blk = table[tok >> p.shift];
@@ -304,32 +310,34 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_rows_kernel(const __grid
                 const long long at = (long long)max(blk, 0) * p.kv_heads + it.h;
                 return blk < 0 ? make_float2(__uint_as_float(kAttnHidden), 0.f) : make_float2(p.ks[at], p.vs[at]);
             };
-            int blk = look(step0), blk1 = look(step0 + 1);
-            float2 f = scales(blk);
-            for (int step = step0; step < step1; ++step, ++n) {
-                const int blk2 = look(step + 2);
-                const float2 f1 = scales(blk1);
-                const int stage = n % Ring::kStages;
-                if (n >= Ring::kStages && !mbar_wait(&empty[stage], ((n / Ring::kStages) - 1) & 1)) {
-                    report_error(ZTQ_ERR_EMPTY_WAIT);
-                    return;
-                }
-                if (lane < 8) info[stage * 8 + lane] = f;
-                const bool copies = lane < 8 && blk >= 0 && (lane & (per - 1)) == 0;
-                const unsigned who = __ballot_sync(0xffffffffu, copies);
-                __syncwarp();                                   // the factors are written before lane 0 arrives
-                if (lane == 0) mbar_expect_tx(&full[stage], __popc(who) * 2 * ((16 * D) << (p.shift - 4)));
-                __syncwarp();
-                if (copies) {
-                    uint8_t* dst = smem + stage * Ring::kStepBytes + 16 * lane * ROW;
-                    const int row = it.h << p.shift;
+            int blk = look(step0);
+            float2 f = scales(blk), f_next = f;
+            for (int first = step0; first < step1; first += 4) {
+                const int blk_next = look(first + 4);
+                for (int k = 0; k < 4 && first + k < step1; ++k, ++n) {
+                    if (k == 2) f_next = scales(blk_next);
+                    const int stage = n % Ring::kStages;
+                    if (n >= Ring::kStages && !mbar_wait(&empty[stage], ((n / Ring::kStages) - 1) & 1)) {
+                        report_error(ZTQ_ERR_EMPTY_WAIT);
+                        return;
+                    }
+                    const bool mine = (lane >> 3) == k, copies = mine && blk >= 0 && (lane & 7 & (per - 1)) == 0;
+                    if (mine) info[stage * 8 + (lane & 7)] = f;
+                    const unsigned who = __ballot_sync(0xffffffffu, copies);
+                    __syncwarp();                               // the factors are written before lane 0 arrives
+                    if (lane == 0) mbar_expect_tx(&full[stage], __popc(who) * 2 * ((16 * D) << (p.shift - 4)));
+                    __syncwarp();
+                    if (copies) {
+                        uint8_t* dst = smem + stage * Ring::kStepBytes + 16 * (lane & 7) * ROW;
+                        const int row = it.h << p.shift;
 #pragma unroll
-                    for (int x = 0; x < D; x += 128) {
-                        tma_load_3d(dst + x * kAttnStep, &k_map, x, row, blk, &full[stage]);
-                        tma_load_3d(dst + kAttnStep * D + x * kAttnStep, &v_map, x, row, blk, &full[stage]);
+                        for (int x = 0; x < D; x += 128) {
+                            tma_load_3d(dst + x * kAttnStep, &k_map, x, row, blk, &full[stage]);
+                            tma_load_3d(dst + kAttnStep * D + x * kAttnStep, &v_map, x, row, blk, &full[stage]);
+                        }
                     }
                 }
-                blk = blk1; blk1 = blk2; f = f1;
+                blk = blk_next; f = f_next;
             }
             w += step1 - step0;
         }
@@ -342,7 +350,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_rows_kernel(const __grid
     auto piece = [](int row, int chunk) {                       // 16-byte piece `chunk` of a row, as the copies swizzle it
         return D == 64 ? row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4) : (chunk >> 3) * (kAttnStep * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
     };
-    int n = 0;
+    int n = 0, mine = warp;                                     // steps so far; the warp's tile of the next one
     for (long long w = w0; w < w_end;) {
         AttnSeq s;
         const AttnItem it = attn_find(p, TILE, upto, w, s);
@@ -403,8 +411,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_rows_kernel(const __grid
         z_max = __reduce_max_sync(0xffffffffu, z_max);
         int vrun = -1000;
 
+        // The CTA's tiles are dealt to the warps in turn, eight per step: `mine` is this warp's tile of the step, if below 8.
+        // A warp without one waits and arrives all the same: a barrier's parity says which phase it is in only to those
+        // who have seen every phase before it.
         for (int step = step0; step < step1; ++step, ++n) {
-            const int stage = n % Ring::kStages, tok = (it.lo / kAttnStep + step) * kAttnStep + 16 * warp;
+            const int stage = n % Ring::kStages, sub = mine, tok = (it.lo / kAttnStep + step) * kAttnStep + 16 * sub;
+            mine += mine < 8 ? kAttnWarps - 8 : -8;
             bool came = !*(volatile int*)&failed;
             if (came && !mbar_wait(&full[stage], (n / Ring::kStages) & 1)) {
                 report_error(ZTQ_ERR_FULL_WAIT);
@@ -412,14 +424,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_rows_kernel(const __grid
                 came = false;
             }
             came = __all_sync(0xffffffffu, came);
-            if (tok >= it.hi || !came) {                        // nothing for this warp
+            if (sub >= 8 || tok >= it.hi || !came) {            // nothing for this warp
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty[stage]);
                 continue;
             }
-            const uint8_t* sk = smem + stage * Ring::kStepBytes + 16 * warp * ROW;
+            const uint8_t* sk = smem + stage * Ring::kStepBytes + 16 * sub * ROW;
             const uint8_t* sv = sk + kAttnStep * D;
-            const float2 f2 = info[stage * 8 + warp];
+            const float2 f2 = info[stage * 8 + sub];
             const bool hidden = __float_as_uint(f2.x) == kAttnHidden;
             // ---- scores of 16 tokens, two chains
             float sc[NT][4], sd[NT][4];
@@ -560,7 +572,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_rows_kernel(const __grid
             if (lane == 0) mbar_arrive(&empty[stage]);
         }
 
-        // ---- the warps' parts meet: 8 -> 4 -> 2 -> 1, in a fixed order
+        // ---- the warps' parts meet, the upper half's with the lower's until one is left, in a fixed order
         {
             const float vref = vrun > -1000 ? ex2((float)vrun) : 0.f;
 #pragma unroll
@@ -574,10 +586,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_rows_kernel(const __grid
                 }
         }
 #pragma unroll
-        for (int half = kAttnWarps / 2; half > 0; half >>= 1) {
+        for (int left = kAttnWarps; left > 1; left = (left + 1) / 2) {
+            const int half = (left + 1) / 2;
             bar_sync(1, 32 * kAttnWarps);                       // what the exchange held before has been read
-            float4* mine = reinterpret_cast<float4*>(swap) + (warp % half) * 32 * (NT * KS + NT) + lane;
-            if (warp >= half && warp < 2 * half) {
+            float4* mine = reinterpret_cast<float4*>(swap) + (warp >= half ? warp - half : warp) * 32 * (NT * KS + NT) + lane;
+            if (warp >= half && warp < left) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     mine[32 * (NT * KS + t)] = make_float4(m[t][0], m[t][1], l[t][0], l[t][1]);
@@ -586,7 +599,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_rows_kernel(const __grid
                 }
             }
             bar_sync(1, 32 * kAttnWarps);
-            if (warp < half) {
+            if (warp + half < left) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     const float4 o = mine[32 * (NT * KS + t)];

@@ -30,9 +30,10 @@ static cudaError_t launch_rows(const AttnParams& p, int sms, cudaStream_t stream
     if (!cache_map(&k_map, p.kc, p, D) || !cache_map(&v_map, p.vc, p, D)) return cudaErrorInvalidValue;
     static std::atomic<unsigned> done{0};
     auto kern = attn_rows_kernel<D, NT, SPLIT>;
-    const int smem = AttnRing<D, NT>::bytes(p.seqs);
-    if (cudaError_t e = allow_smem(kern, done, AttnRing<D, NT>::bytes(kAttnMaxSeqs))) return e;
-    cudaError_t e = launch(kern, dim3(sms), dim3(kAttnThreads), smem, stream, pdl, k_map, v_map, p);
+    using Ring = AttnRing<D, NT, SPLIT>;
+    const int smem = Ring::bytes(p.seqs);
+    if (cudaError_t e = allow_smem(kern, done, Ring::bytes(kAttnMaxSeqs))) return e;
+    cudaError_t e = launch(kern, dim3(sms), dim3(Ring::kThreads), smem, stream, pdl, k_map, v_map, p);
     if (e != cudaSuccess || sms < 2) return e;
     // many parts per row: a CTA per row; else a warp per row
     const bool few = (long long)p.seqs * p.kv_heads <= 32;
