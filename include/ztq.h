@@ -396,7 +396,7 @@ cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_h
  * temperature 0 takes the first of the order.  Per-row arrays; temperature, top_k, top_p, min_p may be NULL (1, all,
  * all, all).  logprob (may be NULL): log of the token's share of what was kept.  -inf and NaN are never drawn; a row
  * with nothing else gives token -1 and logprob NaN.  vocab <= ZTQ_SAMPLE_MAX_VOCAB.  Flags: ZTQ_X_F32, ZTQ_NO_PDL. */
-#define ZTQ_SAMPLE_MAX_VOCAB 389120
+#define ZTQ_SAMPLE_MAX_VOCAB 327680
 cudaError_t ztq_sample(const void* logits, long long row_stride, int rows, int vocab, const float* temperature, const int* top_k,
                        const float* top_p, const float* min_p, const float* uniform, int* token, float* logprob, int flags, cudaStream_t stream);
 

@@ -459,7 +459,7 @@ def sample_rows(x, **kw):
 
 
 @pytest.mark.parametrize("f32", [False, True])
-@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 7), (5, 255), (4, 2049), (64, 1000), (1, 32000), (9, 50257), (2, 131072), (400, 4096), (2, 389120)])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 7), (5, 255), (4, 2049), (64, 1000), (1, 32000), (9, 50257), (2, 131072), (400, 4096), (2, 327680)])
 def test_sample(f32, rows, vocab):
     rng = U.seeded(rows + vocab)
     x = dev(rng.standard_normal((rows, vocab)) * 3, torch.float32 if f32 else torch.float16)

@@ -223,10 +223,12 @@ cudaError_t ztq_sample(const void* logits, long long row_stride, int rows, int v
     if (dev.major < 10) return cudaErrorNoKernelImageForDevice;
     if (rows == 0) return cudaSuccess;
     const bool f32 = flags & ZTQ_X_F32;
-    // CTAs of a row: as many as a slice needs, then as many as keep the device busy while slices stay worth a CTA
+    // CTAs of a row: as many as keep a slice in 64 KB (two CTAs per SM), then twice as many as long as all of them still
+    // run at once and a slice is worth a CTA
     auto slice_of = [&](int ranks) { return ceil_div(ceil_div(vocab, ranks), kSampleSeg) * kSampleSeg; };
     int ranks = 1;
-    while (ranks < kSampleMaxCluster && (slice_of(ranks) > kSampleMaxSlice || ((long long)rows * ranks < 2ll * dev.sms && slice_of(ranks) > 2048))) ranks *= 2;
+    while (ranks < kSampleMaxCluster && slice_of(ranks) * (f32 ? 4 : 2) > 64 * 1024) ranks *= 2;
+    while (ranks < kSampleMaxCluster && (long long)rows * ranks <= dev.sms && slice_of(ranks) > 2048) ranks *= 2;
     SampleParams p{logits, row_stride, temperature, top_k, top_p, min_p, uniform, token, logprob, rows, vocab, slice_of(ranks), ranks,
                    aligned16(logits) && row_stride % (f32 ? 4 : 8) == 0};
     const size_t smem = ((sizeof(SampleShared) + 15) & ~15) + (size_t)p.slice * (f32 ? 4 : 2);

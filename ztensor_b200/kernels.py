@@ -259,24 +259,39 @@ def describe_plan(fmt: str, n: int, k: int, batch: int = 1, group: int = 128, sm
 
 ROPE_PAIRS = 128
 ROPE_SCALING = {"none": 0, "linear": 1, "by_turns": 2, "by_dim": 3}
-SAMPLE_MAX_VOCAB = 389120
+SAMPLE_MAX_VOCAB = 327680
 
 
 def _arg(t, dtype, shape, name):
     """Device pointer of a contiguous tensor of this type and shape on the current device."""
-    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name}: contiguous {dtype} {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}")
-    if not t.is_cuda or t.get_device() != _device():
-        raise ValueError(f"{name}: a tensor on the current CUDA device expected, got one on {t.device}")
-    return t.data_ptr()
+    return _args((dtype, t, shape, name))[0]
+
+
+def _args(*wanted):
+    """Device pointers of (type, tensor, shape, name): contiguous tensors of that type and shape on the current device; 0 for None.
+    One loop with nothing but the checks in it: a step makes dozens of these calls, and they cost more than a small launch."""
+    dev, out = _device(), []
+    for dtype, t, shape, name in wanted:
+        if t is None:
+            out.append(0)
+        elif t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == dev:
+            out.append(t.data_ptr())
+        elif t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name}: contiguous {dtype} {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}")
+        else:
+            raise ValueError(f"{name}: a tensor on the current CUDA device expected, got one on {t.device}")
+    return out
 
 
 def _device():
-    return torch._C._cuda_getDevice()
+    try:
+        return torch._C._cuda_getDevice()
+    except RuntimeError:                        # no device: no tensor is on it
+        return -2
 
 
 def _here(t, name):
-    if not t.is_cuda or t.get_device() != _device():
+    if t.get_device() != _device():
         raise ValueError(f"{name}: a tensor on the current CUDA device expected, got one on {t.device}")
     return t.data_ptr()
 
@@ -330,12 +345,13 @@ class KvCache:
 def kv_plan(ctx_len, new_len, block_table, ring, ring_state, ring_state_out, next_len, kv_len, query_start, positions, slots, status, block_size, flags=0, stream=None):
     """The plan of a step: block table, slots, positions and lengths from the sequences' lengths (ztq_kv_plan).
     All int32; next_len may be ctx_len and ring_state_out may be ring_state."""
-    i, n, rows = torch.int32, ctx_len.shape[0], slots.shape[0]
+    i, n, rows, width, pool = torch.int32, ctx_len.shape[0], slots.shape[0], block_table.shape[-1], ring.shape[0]
+    per_seq, per_row = (n,), (rows,)
     _lib.check(_lib.lib().ztq_kv_plan(
-        _arg(ctx_len, i, (n,), "ctx_len"), _arg(new_len, i, (n,), "new_len"), _arg(block_table, i, (n, block_table.shape[-1]), "block_table"), _arg(ring, i, (ring.numel(),), "ring"),
-        _arg(ring_state, i, (2,), "ring_state"), _arg(ring_state_out, i, (2,), "ring_state_out"), _arg(next_len, i, (n,), "next_len"), _arg(kv_len, i, (n,), "kv_len"),
-        _arg(query_start, i, (n + 1,), "query_start"), _arg(positions, i, (rows,), "positions"), _arg(slots, i, (rows,), "slots"), _arg(status, i, (n,), "status"),
-        n, block_table.shape[1], block_size, ring.shape[0], rows, flags, _stream(stream)), "ztq_kv_plan")
+        *_args((i, ctx_len, per_seq, "ctx_len"), (i, new_len, per_seq, "new_len"), (i, block_table, (n, width), "block_table"), (i, ring, (pool,), "ring"),
+               (i, ring_state, (2,), "ring_state"), (i, ring_state_out, (2,), "ring_state_out"), (i, next_len, per_seq, "next_len"), (i, kv_len, per_seq, "kv_len"),
+               (i, query_start, (n + 1,), "query_start"), (i, positions, per_row, "positions"), (i, slots, per_row, "slots"), (i, status, per_seq, "status")),
+        n, width, block_size, pool, rows, flags, _stream(stream)), "ztq_kv_plan")
 
 
 def rope_table(rows, rot_dim, base, first=0, scaling="none", factor=1.0, turns_low=1.0, turns_high=4.0, original_positions=0, magnitude=1.0, out=None, flags=0, stream=None):
@@ -376,12 +392,10 @@ def rope_append_q8(q, k, v, q_out, slots, cache, table=None, positions=None, fla
         heads = q.shape[1]
         if qf != xf or q.shape[0] != n or q.shape[2] != cache.head_dim or q_out.shape != q.shape:
             raise ValueError(f"q, q_out: {n} rows of heads of {cache.head_dim} and the type of k expected, got {q.dtype} {tuple(q.shape)} and {tuple(q_out.shape)}")
-    tp = pp = rows = rot = 0
-    if table is not None:
-        tp, rows, rot = _arg(table, torch.float32, (*table.shape[:2], 2), "table"), table.shape[0], 2 * table.shape[1]
-        pp = _arg(positions, torch.int32, (n,), "positions")
-    _lib.check(_lib.lib().ztq_rope_append_q8(qp, kp, vp, qo, qt, qh, kt, kh, vt, vh, ot, oh, n, heads, tp, rows, rot, pp, _arg(slots, torch.int32, (n,), "slots"),
-                                             cache._on(), flags | (X_F32 if xf else 0) | (Y_F32 if of else 0), _stream(stream)), "ztq_rope_append_q8")
+    rows, half = table.shape[:2] if table is not None else (0, 0)
+    i = torch.int32
+    tp, pp, sp = _args((torch.float32, table, (rows, half, 2), "table"), (i, positions if table is not None else None, (n,), "positions"), (i, slots, (n,), "slots"))
+    _lib.check(_lib.lib().ztq_rope_append_q8(qp, kp, vp, qo, qt, qh, kt, kh, vt, vh, ot, oh, n, heads, tp, rows, 2 * half, pp, sp, cache._on(), flags | (X_F32 if xf else 0) | (Y_F32 if of else 0), _stream(stream)), "ztq_rope_append_q8")
 
 
 def kv_read_q8(cache, slots, k_out, v_out, flags=0, stream=None):
@@ -389,10 +403,10 @@ def kv_read_q8(cache, slots, k_out, v_out, flags=0, stream=None):
     out = k_out if k_out is not None else v_out
     if out is None or (out.dtype is not torch.float16 and out.dtype is not torch.float32):
         raise ValueError("k_out, v_out: at least one float16 or float32 tensor expected")
-    shape = (slots.shape[0], cache.kv_heads, cache.head_dim)
-    kp, vp = (0 if t is None else _arg(t, out.dtype, shape, name) for t, name in ((k_out, "k_out"), (v_out, "v_out")))
-    _lib.check(_lib.lib().ztq_kv_read_q8(cache._on(), _arg(slots, torch.int32, shape[:1], "slots"), shape[0], kp, vp, flags | (Y_F32 if out.dtype is torch.float32 else 0),
-                                         _stream(stream)), "ztq_kv_read_q8")
+    n = slots.shape[0]
+    shape = (n, cache.kv_heads, cache.head_dim)
+    sp, kp, vp = _args((torch.int32, slots, (n,), "slots"), (out.dtype, k_out, shape, "k_out"), (out.dtype, v_out, shape, "v_out"))
+    _lib.check(_lib.lib().ztq_kv_read_q8(cache._on(), sp, n, kp, vp, flags | (Y_F32 if out.dtype is torch.float32 else 0), _stream(stream)), "ztq_kv_read_q8")
 
 
 def attn_q8_workspace_bytes(tokens, sequences, max_new, q_heads, kv_heads, head_dim) -> int:
@@ -407,11 +421,10 @@ def attn_q8(q, y, query_start, kv_len, block_table, cache, workspace, max_new, s
     seqs = kv_len.shape[0]
     if y.shape != q.shape or dim != cache.head_dim:
         raise ValueError(f"q, y: one shape and heads of {cache.head_dim} expected, got {tuple(q.shape)} and {tuple(y.shape)}")
-    i = torch.int32
-    _lib.check(_lib.lib().ztq_attn_q8(
-        qp, yp, qt, qh, yt, yh, n, heads, _arg(query_start, i, (seqs + 1,), "query_start"), _arg(kv_len, i, (seqs,), "kv_len"), _arg(block_table, i, (seqs, block_table.shape[-1]), "block_table"),
-        seqs, block_table.shape[1], max_new, window, C.c_uint.from_buffer(C.c_float(scale)).value, cache._on(), _here(workspace, "workspace"), workspace.numel() * workspace.element_size(),
-        flags | (X_F32 if xf else 0) | (Y_F32 if yf else 0), _stream(stream)), "ztq_attn_q8")
+    i, width = torch.int32, block_table.shape[-1]
+    sp, lp, bp = _args((i, query_start, (seqs + 1,), "query_start"), (i, kv_len, (seqs,), "kv_len"), (i, block_table, (seqs, width), "block_table"))
+    _lib.check(_lib.lib().ztq_attn_q8(qp, yp, qt, qh, yt, yh, n, heads, sp, lp, bp, seqs, width, max_new, window, C.c_uint.from_buffer(C.c_float(scale)).value, cache._on(),
+                                      _here(workspace, "workspace"), workspace.nbytes, flags | (X_F32 if xf else 0) | (Y_F32 if yf else 0), _stream(stream)), "ztq_attn_q8")
 
 
 def sample(logits, uniform, token, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None, flags=0, stream=None):
@@ -419,8 +432,8 @@ def sample(logits, uniform, token, logprob=None, temperature=None, top_k=None, t
     if logits.dim() != 2 or (logits.dtype is not torch.float16 and logits.dtype is not torch.float32) or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError(f"logits: float16 or float32 [rows, vocab] with contiguous rows expected, got {logits.dtype} {tuple(logits.shape)}, strides {logits.stride()}")
     n, vocab = logits.shape
-    f, i = torch.float32, torch.int32
-    opt = lambda t, dtype, name: 0 if t is None else _arg(t, dtype, (n,), name)  # noqa: E731
-    _lib.check(_lib.lib().ztq_sample(_here(logits, "logits"), logits.stride(0) if n > 1 else 0, n, vocab, opt(temperature, f, "temperature"), opt(top_k, i, "top_k"), opt(top_p, f, "top_p"),
-                                     opt(min_p, f, "min_p"), _arg(uniform, f, (n,), "uniform"), _arg(token, i, (n,), "token"), opt(logprob, f, "logprob"),
-                                     flags | (X_F32 if logits.dtype is torch.float32 else 0), _stream(stream)), "ztq_sample")
+    f, i, rows = torch.float32, torch.int32, (n,)
+    _lib.check(_lib.lib().ztq_sample(
+        _here(logits, "logits"), logits.stride(0) if n > 1 else 0, n, vocab,
+        *_args((f, temperature, rows, "temperature"), (i, top_k, rows, "top_k"), (f, top_p, rows, "top_p"), (f, min_p, rows, "min_p"), (f, uniform, rows, "uniform"), (i, token, rows, "token"),
+               (f, logprob, rows, "logprob")), flags | (X_F32 if logits.dtype is torch.float32 else 0), _stream(stream)), "ztq_sample")
