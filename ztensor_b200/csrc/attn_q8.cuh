@@ -136,7 +136,10 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
 }
 
 // Where CTA i's range of `total` steps begins when `ctas` of them share it.
-__device__ __forceinline__ long long attn_cut(long long total, int i, int ctas) { return total * i / ctas; }
+// (divisions in 64 bits take hundreds of clocks each, and stand in front of everything else)
+__device__ __forceinline__ long long attn_cut(long long total, int i, int ctas) {
+    return total < (1 << 20) ? (unsigned)total * (unsigned)i / (unsigned)ctas : total * i / ctas;      // ctas < 2^12
+}
 __device__ __forceinline__ int attn_ctas(long long total, int grid) {
     const long long n = (total + kAttnMinSteps - 1) / kAttnMinSteps;
     return (int)max(1ll, min(n, (long long)grid));
@@ -204,7 +207,8 @@ __device__ __forceinline__ AttnItem attn_find(const AttnParams& p, int tile, con
         if (w < it.begin + n || it.r1 >= rows) break;
         it.begin += n;
     }
-    it.h = (int)((w - it.begin) / it.steps);
+    const long long ahead = w - it.begin;
+    it.h = ahead < 0x7fffffff ? (int)((unsigned)ahead / (unsigned)it.steps) : (int)(ahead / it.steps);
     it.begin += (long long)it.h * it.steps;
     return it;
 }
@@ -322,12 +326,8 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
                         return;
                     }
                     const bool mine = (lane >> 3) == k, copies = mine && blk >= 0 && (lane & 7 & (per - 1)) == 0;
-                    if (mine) info[stage * 8 + (lane & 7)] = f;
                     const unsigned who = __ballot_sync(0xffffffffu, copies);
-                    __syncwarp();                               // the factors are written before lane 0 arrives
-                    if (lane == 0) mbar_expect_tx(&full[stage], __popc(who) * 2 * ((16 * D) << (p.shift - 4)));
-                    __syncwarp();
-                    if (copies) {
+                    if (copies) {                               // ahead of the arrival, which keeps the phase open: the factors may still be on their way
                         uint8_t* dst = smem + stage * Ring::kStepBytes + 16 * (lane & 7) * ROW;
                         const int row = it.h << p.shift;
 #pragma unroll
@@ -336,6 +336,9 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
                             tma_load_3d(dst + kAttnStep * D + x * kAttnStep, &v_map, x, row, blk, &full[stage]);
                         }
                     }
+                    if (mine) info[stage * 8 + (lane & 7)] = f;
+                    __syncwarp();                               // the factors are written before lane 0 arrives
+                    if (lane == 0) mbar_expect_tx(&full[stage], __popc(who) * 2 * ((16 * D) << (p.shift - 4)));
                 }
                 blk = blk_next; f = f_next;
             }
@@ -679,7 +682,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnParam
     if (!cuts || it.begin == w || attn_cut(total, cta, ctas) > it.begin) return;     // no cut inside, or not the first one
     // CTAs cta .. cta + n - 1 hold parts; the last is the one whose range reaches the item's end
     const long long end = it.begin + it.steps;
-    int last = (int)(end * ctas / total);
+    int last = end < (1 << 20) ? (int)((unsigned)end * (unsigned)ctas / (unsigned)total) : (int)(end * ctas / total);
     while (last > cta && attn_cut(total, last, ctas) >= end) --last;
     while (attn_cut(total, last + 1, ctas) < end) ++last;
     const int n = last - cta + 1, r = share == 1 ? blockIdx.y * WARPS + warp : blockIdx.y;

@@ -12,10 +12,14 @@
 // A power of two makes x / scale' exact, so the only rounding is the one to a code (half a step), and growth costs the
 // old rows at most the half step they are entitled to at the new scale.  A non-finite new row makes the scale NaN.
 //
-// Work: units of 16 elements of one head.  A CTA holds a tile of kTokenTile rows; blockIdx.y is a group of query heads
-// or a key/value head.  The rows of one block stand together (a run); the CTA whose tile holds a run's first row does
-// the whole run, so a block has one writer and needs no atomics.  With few runs in the tile (a prompt) the CTA's warps
-// share each run, with many (decoding) every warp takes runs of its own.
+// Work: units of 16 elements of one head.  A CTA holds a tile of kTokenTile rows, for a group of query heads or for the
+// keys or values of one head.  Queries: a thread keeps one (row, unit) and its eight cosines and sines and goes through the heads.
+// The rows of one block stand together (a run); the CTA whose tile holds a run's first row does the whole run, so a block
+// has one writer and needs no atomics.  Keys and values are two CTAs.  With few runs in the tile (a prompt) the whole CTA
+// takes each run, with many (decoding) every warp takes runs of its own.  The rows are read twice, for the largest value
+// and for the rounding; the second time they come from L1 (holding them in registers cost the queries' part its occupancy).
+// A prompt is bound by HBM (8192 rows, 32 + 8 + 8 heads of 128 in fp16: 186 MB), a decode step by the chain
+// slot -> scale and codes -> store.
 #pragma once
 
 #include "ztq_common.cuh"
@@ -23,7 +27,8 @@
 namespace ztq {
 
 constexpr int kRopeThreads = 256;
-constexpr int kTokenTile = 16;
+constexpr int kTokenTile = 16;                     // rows of a tile of queries
+constexpr int kMaxKvTile = 64;                     // of keys and values: 64 for many rows, where most tiles of 16 would begin no run
 
 struct RopeParams {
     const float2* table;       // [table_rows][half]; NULL: no rotation
@@ -47,6 +52,7 @@ struct AppendParams {
     long long block_stride;    // bytes
     int blocks, kv_heads, shift, dim, tokens, q_heads;
     int q_groups, q_group;     // groups of query heads, heads in one
+    int q_ctas, kv_tile;       // CTAs of the queries' part, which come last
     int x_f32, y_f32, vec;     // vec: pointers and strides allow 16-byte accesses
     RopeParams rope;
 };
@@ -115,8 +121,7 @@ __device__ __forceinline__ void unit_offsets(const RopeParams& r, int j, int& e0
     else { e0 = 16 * j; e1 = 16 * j + 8; }              // pairs, and what lies behind the rotated part
 }
 
-__device__ __forceinline__ void rotate_unit(const RopeParams& r, const float2* row, int j, float (&a)[8], float (&b)[8]) {
-    float2 cs[8];
+__device__ __forceinline__ void load_turn(const float2* row, int j, float2 (&cs)[8]) {
     if (row) {
         const float4* s = reinterpret_cast<const float4*>(row + 8 * j);
 #pragma unroll
@@ -130,7 +135,10 @@ __device__ __forceinline__ void rotate_unit(const RopeParams& r, const float2* r
 #pragma unroll
         for (int i = 0; i < 8; ++i) cs[i] = make_float2(nan, nan);
     }
-    if (r.pairs) {
+}
+
+__device__ __forceinline__ void rotate_unit(bool pairs, const float2 (&cs)[8], float (&a)[8], float (&b)[8]) {
+    if (pairs) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float x0 = a[2 * i], y0 = a[2 * i + 1], x1 = b[2 * i], y1 = b[2 * i + 1];
@@ -149,9 +157,8 @@ __device__ __forceinline__ void rotate_unit(const RopeParams& r, const float2* r
     }
 }
 
-// The table row of a token; NULL (the rotated part becomes NaN) where its position lies outside the table.
-__device__ __forceinline__ const float2* rope_row(const RopeParams& r, int token) {
-    const int pos = r.positions[token];
+// The table row of a position; NULL (the rotated part becomes NaN) where it lies outside the table.
+__device__ __forceinline__ const float2* rope_row(const RopeParams& r, int pos) {
     if (pos < 0 || pos >= r.table_rows) {
         report_error(ZTQ_ERR_POSITION);
         return nullptr;
@@ -161,25 +168,29 @@ __device__ __forceinline__ const float2* rope_row(const RopeParams& r, int token
 
 template <bool XF32, bool YF32>
 __device__ __forceinline__ void rope_heads(const RopeParams& r, const HeadsIn& x, const HeadsIn& y, int t0, int t1, int h0, int h1, int dim, bool vec) {
-    const int units = dim >> 4, heads = h1 - h0;
-    for (int i = threadIdx.x; i < (t1 - t0) * heads * units; i += blockDim.x) {
-        const int j = i % units, h = h0 + i / units % heads, t = t0 + i / (units * heads);
-        int e0, e1;
-        bool rotated;
-        unit_offsets(r, j, e0, e1, rotated);
-        const long long src = t * x.token + h * x.head, dst = t * y.token + h * y.head;
+    const int units = dim >> 4, pairs = kTokenTile * units, strides = kRopeThreads / pairs;      // threads of one head: at most the CTA's
+    const int at = threadIdx.x % pairs, j = at % units, t = t0 + at / units, first = threadIdx.x / pairs;
+    if (first >= strides || t >= t1) return;
+    int e0, e1;
+    bool rotated;
+    unit_offsets(r, j, e0, e1, rotated);
+    float2 cs[8];
+    if (rotated) load_turn(rope_row(r, r.positions[t]), j, cs);
+    const long long src = t * x.token, dst = t * y.token;
+#pragma unroll 4
+    for (int h = h0 + first; h < h1; h += strides) {
         float a[8], b[8];
-        load8<XF32>(x.p, src + e0, vec, a);
-        load8<XF32>(x.p, src + e1, vec, b);
-        if (rotated) rotate_unit(r, rope_row(r, t), j, a, b);
-        store8<YF32>(const_cast<void*>(y.p), dst + e0, vec, a);
-        store8<YF32>(const_cast<void*>(y.p), dst + e1, vec, b);
+        load8<XF32>(x.p, src + h * x.head + e0, vec, a);
+        load8<XF32>(x.p, src + h * x.head + e1, vec, b);
+        if (rotated) rotate_unit(r.pairs, cs, a, b);
+        store8<YF32>(const_cast<void*>(y.p), dst + h * y.head + e0, vec, a);
+        store8<YF32>(const_cast<void*>(y.p), dst + h * y.head + e1, vec, b);
     }
 }
 
 // A unit of a new row of keys (rotated) or values.
 template <bool XF32>
-__device__ __forceinline__ void append_unit(const AppendParams& p, bool key, int t, int h, int j, float (&a)[8], float (&b)[8], int& e0, int& e1) {
+__device__ __forceinline__ void append_unit(const AppendParams& p, bool key, int t, int pos, int h, int j, float (&a)[8], float (&b)[8], int& e0, int& e1) {
     const HeadsIn& x = key ? p.k : p.v;
     bool rotated = false;
     if (key) unit_offsets(p.rope, j, e0, e1, rotated);
@@ -187,17 +198,19 @@ __device__ __forceinline__ void append_unit(const AppendParams& p, bool key, int
     const long long src = t * x.token + h * x.head;
     load8<XF32>(x.p, src + e0, p.vec, a);
     load8<XF32>(x.p, src + e1, p.vec, b);
-    if (rotated) rotate_unit(p.rope, rope_row(p.rope, t), j, a, b);
+    if (rotated) {
+        float2 cs[8];
+        load_turn(rope_row(p.rope, pos), j, cs);
+        rotate_unit(p.rope.pairs, cs, a, b);
+    }
 }
 
-__device__ __forceinline__ uint32_t pack4(const float* v, float inv, bool dead) {
-    uint32_t w = 0;
+// Four codes of v * inv, rounded to nearest even: adding 1.5 2^23 leaves the integer in the low byte.
+__device__ __forceinline__ uint32_t pack4(const float* v, float inv) {
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = dead ? 0 : __float2int_rn(fminf(fmaxf(v[i] * inv, -127.f), 127.f));
-        w |= (uint32_t)(c & 255) << (8 * i);
-    }
-    return w;
+    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(fminf(fmaxf(v[i] * inv, -127.f), 127.f) + 12582912.f);
+    return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
 }
 
 // The smallest power of two s with amax <= 127 s (not below the smallest normal number); NaN for a non-finite amax.
@@ -208,20 +221,22 @@ __device__ __forceinline__ float scale_for(float amax) {
     return __uint_as_float((uint32_t)max(e, 1) << 23);
 }
 
-// One run (rows t0 .. t0 + n of a block, from offset `off` of it) of one head, keys or values, by a group of `lanes`
-// threads (a warp, or the whole CTA with its shared word `red`).
-template <bool XF32>
-__device__ __forceinline__ void append_run(const AppendParams& p, bool key, int h, int t0, int n, int block, int off, int lane, int lanes, float* red) {
-    const int units = p.dim >> 4, size = 1 << p.shift;
+// One run (rows t0 .. t0 + n of a block, from offset `off` of it, at positions pos[0 .. n)) of one head, keys or values, by
+// LANES threads: a warp, or the whole CTA with its shared words `red`.
+template <bool XF32, int LANES>
+__device__ __forceinline__ void append_run(const AppendParams& p, bool key, int h, int t0, const int* pos, int n, int block, int off, int lane, float* red) {
+    const int units = p.dim >> 4, size = 1 << p.shift, items = n * units;
     int8_t* codes = (key ? p.kc : p.vc) + block * p.block_stride + (long long)h * size * p.dim;
     float* scale_at = (key ? p.ks : p.vs) + (long long)block * p.kv_heads + h;
-    const float had = *scale_at;
+    const float had = off > 0 ? *scale_at : 0.f;
     float amax = 0.f;
     bool odd = false;                                  // a NaN: fmaxf would drop it
     int e0, e1;
-    for (int i = lane; i < n * units; i += lanes) {
+#pragma unroll 2
+    for (int i = lane; i < items; i += LANES) {
         float a[8], b[8];
-        append_unit<XF32>(p, key, t0 + i / units, h, i % units, a, b, e0, e1);
+        const int t = i / units;
+        append_unit<XF32>(p, key, t0 + t, pos[t], h, i - t * units, a, b, e0, e1);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             amax = fmaxf(amax, fmaxf(fabsf(a[k]), fabsf(b[k])));
@@ -231,11 +246,12 @@ __device__ __forceinline__ void append_run(const AppendParams& p, bool key, int 
     if (odd) amax = __int_as_float(0x7f800000);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (lanes > 32) {
-        __syncthreads();                               // the previous run's readers are done with red, and everyone has read `had`
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+    if constexpr (LANES > 32) {
+        __syncthreads();                               // the previous run's readers are done with red; everyone has read `had`
+        if ((lane & 31) == 0) red[lane >> 5] = amax;
         __syncthreads();
-        for (int w = 0; w < (lanes >> 5); ++w) amax = fmaxf(amax, red[w]);
+#pragma unroll
+        for (int w = 0; w < LANES / 32; ++w) amax = fmaxf(amax, red[w]);
     }
     const float need = scale_for(amax);
     float scale = need;
@@ -243,7 +259,7 @@ __device__ __forceinline__ void append_run(const AppendParams& p, bool key, int 
     const bool dead = scale != scale;
     if (off > 0 && !dead && scale != had) {            // the block's scale grows: its rows are rounded to the new step
         const float ratio = had / scale;
-        for (int i = lane; i < off * units; i += lanes) {
+        for (int i = lane; i < off * units; i += LANES) {
             uint4 w = *reinterpret_cast<const uint4*>(codes + 16 * i);
             uint32_t* q = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
@@ -251,69 +267,75 @@ __device__ __forceinline__ void append_run(const AppendParams& p, bool key, int 
                 float v[4];
 #pragma unroll
                 for (int m = 0; m < 4; ++m) v[m] = (float)(int8_t)(q[k] >> (8 * m));
-                q[k] = pack4(v, ratio, false);
+                q[k] = pack4(v, ratio);
             }
             *reinterpret_cast<uint4*>(codes + 16 * i) = w;
         }
     }
-    // 1 / scale of a power of two is exact, but below 2^-126 for the largest scales: division by it is not
+    // A power of two's reciprocal is exact; a scale from elsewhere that stays (the append writes powers of two) costs one
+    // more rounding of 2^-24.  Dead blocks get code 0.
     const float inv = 1.f / scale;
-    for (int i = lane; i < n * units; i += lanes) {
+    for (int i = lane; i < items; i += LANES) {
         float a[8], b[8];
         const int t = i / units;
-        append_unit<XF32>(p, key, t0 + t, h, i % units, a, b, e0, e1);
+        append_unit<XF32>(p, key, t0 + t, pos[t], h, i - t * units, a, b, e0, e1);
         int8_t* row = codes + (long long)(off + t) * p.dim;
-        *reinterpret_cast<uint2*>(row + e0) = make_uint2(pack4(a, inv, dead), pack4(a + 4, inv, dead));
-        *reinterpret_cast<uint2*>(row + e1) = make_uint2(pack4(b, inv, dead), pack4(b + 4, inv, dead));
+        *reinterpret_cast<uint2*>(row + e0) = dead ? make_uint2(0, 0) : make_uint2(pack4(a, inv), pack4(a + 4, inv));
+        *reinterpret_cast<uint2*>(row + e1) = dead ? make_uint2(0, 0) : make_uint2(pack4(b, inv), pack4(b + 4, inv));
     }
     if (lane == 0) *scale_at = scale;
 }
 
 template <bool XF32, bool YF32>
-__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const AppendParams p) {
-    __shared__ int s_run[kTokenTile], s_count;
+__global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const AppendParams p) {
+    constexpr int kSeen = kMaxKvTile + 128;            // rows that a run of the tile may reach
+    __shared__ int s_slot[kSeen + 1], s_pos[kSeen], s_run[kMaxKvTile], s_count;
     __shared__ float red[kRopeThreads / 32];
     grid_dep_launch();
     grid_dep_wait();
-    const int t0 = blockIdx.x * kTokenTile, t1 = min(t0 + kTokenTile, p.tokens);
-    if ((int)blockIdx.y < p.q_groups) {
-        const int h0 = blockIdx.y * p.q_group;
-        rope_heads<XF32, YF32>(p.rope, p.q, p.qo, t0, t1, h0, min(h0 + p.q_group, p.q_heads), p.dim, p.vec);
+    const int kv_parts = 2 * p.kv_heads, kv_ctas = (int)gridDim.x - p.q_ctas;
+    if ((int)blockIdx.x >= kv_ctas) {
+        const int at = blockIdx.x - kv_ctas, t0 = at / p.q_groups * kTokenTile, h0 = at % p.q_groups * p.q_group;
+        rope_heads<XF32, YF32>(p.rope, p.q, p.qo, t0, min(t0 + kTokenTile, p.tokens), h0, min(h0 + p.q_group, p.q_heads), p.dim, p.vec);
         return;
     }
-    const int h = blockIdx.y - p.q_groups, size = 1 << p.shift;
+    const int tile = blockIdx.x / kv_parts, which = blockIdx.x % kv_parts, t0 = tile * p.kv_tile;
+    const int h = which >> 1, size = 1 << p.shift, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool key = !(which & 1);
     const long long limit = (long long)p.blocks << p.shift;
-    if (threadIdx.x < 32) {
-        // rows of this tile that begin a run
-        const int t = t0 + threadIdx.x;
-        bool begins = false;
-        if (threadIdx.x < kTokenTile && t < t1) {
-            const int s = p.slots[t], before = t > 0 ? p.slots[t - 1] : -1;
-            begins = s >= 0 && s < limit;
-            if (s >= limit) report_error(ZTQ_ERR_SLOT);
-            if (begins && before >= 0 && (before >> p.shift) == (s >> p.shift)) {
-                begins = false;
-                if (s != before + 1) report_error(ZTQ_ERR_SLOT);           // and append_run's count stops in front of it
-            }
+    // slots and positions of all rows that matter here, in one go; s_slot[0] is the row in front of the tile
+    if (tid < p.kv_tile + size && tid < kSeen) {
+        const int t = t0 + tid;
+        s_slot[tid + 1] = t < p.tokens ? p.slots[t] : -1;
+        s_pos[tid] = key && p.rope.table && t < p.tokens ? p.rope.positions[t] : 0;
+    }
+    if (tid == kRopeThreads - 1) { s_slot[0] = t0 > 0 ? p.slots[t0 - 1] : -1; s_count = 0; }
+    __syncthreads();
+    if (tid < p.kv_tile) {                             // rows of this tile that begin a run
+        const int s = s_slot[tid + 1], before = s_slot[tid];
+        bool begins = s >= 0 && s < limit;
+        if (s >= limit) report_error(ZTQ_ERR_SLOT);
+        if (begins && before >= 0 && (before >> p.shift) == (s >> p.shift)) {
+            begins = false;
+            if (s != before + 1) report_error(ZTQ_ERR_SLOT);               // and the run in front ends there
         }
-        const unsigned found = __ballot_sync(0xffffffffu, begins);
-        if (begins) s_run[__popc(found & ((1u << threadIdx.x) - 1))] = t;
-        if (threadIdx.x == 0) s_count = __popc(found);
+        if (begins) s_run[atomicAdd(&s_count, 1)] = tid;
     }
     __syncthreads();
-    const int runs = s_count, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool shared = 2 * runs < kRopeThreads / 32;
-    for (int i = shared ? 0 : warp; i < 2 * runs; i += shared ? 1 : kRopeThreads / 32) {
-        const int t = s_run[i >> 1], s = p.slots[t], off = s & (size - 1);
+    const int runs = s_count;
+    const bool shared = runs < kRopeThreads / 32;
+    for (int i = shared ? 0 : warp; i < runs; i += shared ? 1 : kRopeThreads / 32) {
+        const int at = s_run[i], s = s_slot[at + 1], off = s & (size - 1);
         int n = 1;                                     // rows of the run: 32 candidates at a time
         while (off + n < size) {
-            const int u = t + n + lane;
-            const bool goes_on = u < p.tokens && off + n + lane < size && p.slots[u] == s + n + lane;
+            const int u = n + lane;
+            const bool goes_on = off + u < size && s_slot[at + 1 + u] == s + u;
             const unsigned miss = ~__ballot_sync(0xffffffffu, goes_on);
             n += miss ? __ffs(miss) - 1 : 32;
             if (miss) break;
         }
-        append_run<XF32>(p, !(i & 1), h, t, n, s >> p.shift, off, shared ? threadIdx.x : lane, shared ? kRopeThreads : 32, red);
+        if (shared) append_run<XF32, kRopeThreads>(p, key, h, t0 + at, s_pos + at, n, s >> p.shift, off, tid, red);
+        else append_run<XF32, 32>(p, key, h, t0 + at, s_pos + at, n, s >> p.shift, off, lane, red);
     }
 }
 
@@ -348,9 +370,11 @@ __global__ void __launch_bounds__(kRopeThreads) kv_read_kernel(const AppendParam
     grid_dep_launch();
     grid_dep_wait();
     const int units = p.dim >> 4, size = 1 << p.shift;
-    const long long per = (long long)p.kv_heads * units, n = p.tokens * per, limit = (long long)p.blocks << p.shift;
+    const int per = p.kv_heads * units;
+    const long long n = (long long)p.tokens * per, limit = (long long)p.blocks << p.shift;
     for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        const int t = (int)(i / per), h = (int)(i % per) / units, j = (int)(i % units);
+        const int t = n < 0x7fffffff ? (int)((unsigned)i / (unsigned)per) : (int)(i / per);     // a 64-bit division costs more than the copy
+        const int rest = (int)(i - (long long)t * per), h = rest / units, j = rest % units;
         const int s = p.slots[t];
         if (s < 0 || s >= limit) continue;
         const int block = s >> p.shift;

@@ -7,6 +7,7 @@
 #include "rope_append.cuh"
 #include "sample.cuh"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -50,9 +51,9 @@ static bool wide(const HeadsIn& x, bool f32) {
     return aligned16(x.p) && x.token % n == 0 && x.head % n == 0;
 }
 
-// Query heads a CTA takes: enough groups to fill the device when there are few tokens
+// Query heads a CTA takes: all of them once the row tiles fill the device, else as few as its threads hold at a time
 static int head_group(int heads, int tiles, int dim, int sms) {
-    const int least = 256 / dim > 0 ? 256 / dim : 1;      // a CTA's 256 threads hold 16 rows of 256 elements
+    const int least = std::max(1, kRopeThreads / (kTokenTile * (dim / 16)));
     int group = heads;
     while (group > least && (long long)tiles * ceil_div(heads, group) < 4ll * sms) group = (group + 1) / 2;
     return group;
@@ -180,10 +181,13 @@ cudaError_t ztq_rope_append_q8(const void* q, const void* k, const void* v, void
     p.y_f32 = yf;
     p.vec = wide(p.k, xf) && wide(p.v, xf) && (q_heads == 0 || (wide(p.q, xf) && wide(p.qo, yf)));
     const int tiles = ceil_div(tokens, kTokenTile);
-    p.q_group = q_heads ? max(head_group(q_heads, tiles, p.dim, dev.sms), ceil_div(q_heads, 32767)) : 1;
+    p.q_group = q_heads ? head_group(q_heads, tiles, p.dim, dev.sms) : 1;
     p.q_groups = q_heads ? ceil_div(q_heads, p.q_group) : 0;
-    if (p.q_groups + p.kv_heads > 65535) return cudaErrorInvalidValue;
-    const dim3 grid(tiles, p.q_groups + p.kv_heads);
+    p.kv_tile = tokens >= 16 * kMaxKvTile ? kMaxKvTile : kTokenTile;
+    const long long q_ctas = (long long)tiles * p.q_groups, ctas = q_ctas + (long long)ceil_div(tokens, p.kv_tile) * 2 * p.kv_heads;
+    if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+    p.q_ctas = (int)q_ctas;
+    const dim3 grid((unsigned)ctas);
     auto kern = xf ? (yf ? rope_append_kernel<true, true> : rope_append_kernel<true, false>) : (yf ? rope_append_kernel<false, true> : rope_append_kernel<false, false>);
     cudaError_t e = launch(kern, grid, dim3(kRopeThreads), 0, stream, !(flags & ZTQ_NO_PDL), p);
     return e != cudaSuccess ? e : cudaGetLastError();
