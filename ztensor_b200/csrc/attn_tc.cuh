@@ -10,8 +10,8 @@
 // the step's largest, V codes by theirs over a power of two near the step's largest, so that one factor per step remains
 // (exact for the powers of two that the append writes; other scales are rounded to fp16).
 //
-// Roles of the 17 warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread is a row: TMEM lane), 8-15 codes -> operands
-// (warp w: keys 16 w .. 16 w + 15 of a step), 16 issues the products.  The two tiles alternate: while one is in its softmax
+// Roles of the 17 warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread is a row: TMEM lane), 8-11 K codes -> operand, 12-15
+// V codes (32 keys of a step each, loaded one step ahead, their blocks and scales two), 16 issues the products.  The two tiles alternate: while one is in its softmax
 // the tensor cores work for the other.  The running maximum moves only when a score exceeds it by more than kAttnSlack
 // (then the row's O is rescaled in TMEM), as does the reference of the V scales.
 // Operands stand in the canonical K-major layout without swizzle: core matrices of 8 rows x 16 bytes, 128 bytes apart along
@@ -26,6 +26,8 @@
 
 #include "attn_q8.cuh"
 #include "tc_common.cuh"
+
+#include <type_traits>
 
 namespace ztq {
 
@@ -158,11 +160,11 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.k_full[i], 8); mbar_init(&sh.k_empty[i], 1);
-            mbar_init(&sh.v_full[i], 8); mbar_init(&sh.v_empty[i], 1);
+            mbar_init(&sh.k_full[i], 4); mbar_init(&sh.k_empty[i], 1);
+            mbar_init(&sh.v_full[i], 4); mbar_init(&sh.v_empty[i], 1);
             mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 128); mbar_init(&sh.o_full[i], 1);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(&sh.info_full[i], 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&sh.info_full[i], 2);
         mbar_fence_init();
     }
     if (warp == 16) {
@@ -203,123 +205,135 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
     };
 
     if (warp >= 8 && warp < 16) {
-        // ------------------------------------------------ codes -> operands
-        const int w = warp - 8;
+        // ------------------------------------------------ codes -> operands: warps 8-11 K, 12-15 V, 32 keys each
+        const bool is_k = warp < 12;
+        const int w = (warp & 3) * 2;                             // first of the warp's two groups of 16 keys
         const int* table = p.block_table + (long long)it.b * p.width;
         constexpr int KL = D / 64, LR = D / 4, VG = LR / 16;      // 16-byte loads per key and lane; lanes per row of V, key groups per lane
         const int vg = lane / LR, vd = lane % LR;                 // V: first key group, word of four dims
         const int rot = (vd >> 1) & 3;
         auto sel = [](int a, int b) { return (uint32_t)(a | (4 + a) << 4 | b << 8 | (4 + b) << 12); };
         const uint32_t sel0 = sel(rot, (rot + 1) & 3), sel1 = sel((rot + 2) & 3, (rot + 3) & 3);
-        uint4 kb[2][KL];
-        uint32_t vb[VG][8];
-        float ks = 0.f, vs = 0.f;                                 // of group `lane & 7` of the step
-        int blk = -1;                                             // ditto
-        auto load = [&](int kt) {
-            // every lane looks up group (lane & 7): all groups' scales are known to all warps
+        uint64_t* full = is_k ? sh.k_full : sh.v_full;
+        uint64_t* empty = is_k ? sh.k_empty : sh.v_empty;
+        const float* scales = is_k ? p.ks : p.vs;
+        const int8_t* codes = is_k ? p.kc : p.vc;
+        // every lane looks up group (lane & 7): all groups' blocks and scales are known to all warps
+        auto look = [&](int kt) {
             const int tok = kt * kTcaKeys + 16 * (lane & 7);
-            blk = -1;
-            ks = vs = 0.f;
-            if (tok < it.hi) {
+            int blk = -1;
+            if (kt < kt1 && tok < it.hi) {
                 blk = table[tok >> p.shift];
                 if ((unsigned)blk >= (unsigned)p.blocks) {
                     report_error(ZTQ_ERR_BLOCK);
                     blk = -1;
-                } else {
-                    ks = p.ks[(long long)blk * p.kv_heads + it.h];
-                    vs = p.vs[(long long)blk * p.kv_heads + it.h];
                 }
             }
-            const int own = __shfl_sync(0xffffffffu, blk, w);
-            const int at = (kt * kTcaKeys + 16 * w) & ((1 << p.shift) - 1);
-            const long long off = max(own, 0) * p.block_stride + (((long long)it.h << p.shift) + at) * D;
-            if (own >= 0) {
+            return blk;
+        };
+        auto scale_of = [&](int blk) { return blk >= 0 ? scales[(long long)blk * p.kv_heads + it.h] : 0.f; };
+        uint4 raw[2][2 * KL];                                     // 16 keys' codes of this lane, twice
+        auto load = [&](int kt, int blks) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+            for (int g = 0; g < 2; ++g) {
+                const int own = __shfl_sync(0xffffffffu, blks, w + g);
+                const int at = (kt * kTcaKeys + 16 * (w + g)) & ((1 << p.shift) - 1);
+                const int8_t* src = codes + max(own, 0) * p.block_stride + (((long long)it.h << p.shift) + at) * D;
+                if (own < 0) {
 #pragma unroll
-                    for (int j = 0; j < KL; ++j) kb[i][j] = ld_stream(p.kc + off + ((lane & 7) + 8 * i) * D + 16 * ((lane >> 3) + 4 * j));
+                    for (int i = 0; i < 2 * KL; ++i) raw[g][i] = make_uint4(0, 0, 0, 0);
+                } else if (is_k) {                                // key (lane & 7) + 8 a, piece lane / 8 + 4 j
 #pragma unroll
-                for (int g = 0; g < VG; ++g)
+                    for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) vb[g][i] = __ldg(reinterpret_cast<const uint32_t*>(p.vc + off + (8 * (vg + g) + i) * D + 4 * vd));
-            } else {
+                        for (int j = 0; j < KL; ++j) raw[g][a * KL + j] = ld_stream(src + ((lane & 7) + 8 * a) * D + 16 * ((lane >> 3) + 4 * j));
+                } else {                                          // four dims of eight keys, VG times
+                    uint32_t* r = reinterpret_cast<uint32_t*>(&raw[g][0]);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                    for (int v = 0; v < VG; ++v)
 #pragma unroll
-                    for (int j = 0; j < KL; ++j) kb[i][j] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int g = 0; g < VG; ++g)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) vb[g][i] = 0;
+                        for (int i = 0; i < 8; ++i) r[8 * v + i] = __ldg(reinterpret_cast<const uint32_t*>(src + (8 * (vg + v) + i) * D + 4 * vd));
+                }
             }
         };
-        if (n > 0) load(kt0);
+        int blk = look(kt0), blk1 = look(kt0 + 1);
+        float sc = scale_of(blk);
+        if (n > 0) load(kt0, blk);
         for (int i = 0; i < n; ++i) {
             const int slot = i & 1;
+            const int blk2 = look(kt0 + i + 2);                   // two steps ahead, scales one: their loads wait for one another
+            const float sc1 = scale_of(blk1);
             // factors of the step
-            const bool fine_v = fabsf(vs) <= 3.402823466e38f;
-            float kref = fabsf(ks) <= 3.402823466e38f ? fabsf(ks) : 0.f;
-            uint32_t vtop = fine_v ? __float_as_uint(fabsf(vs)) >> 23 : 0u;
+            const bool fine = fabsf(sc) <= 3.402823466e38f;
+            float kref = fine ? fabsf(sc) : 0.f;
+            uint32_t top = fine ? __float_as_uint(fabsf(sc)) >> 23 : 0u;
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) {
                 kref = fmaxf(kref, __shfl_xor_sync(0xffffffffu, kref, o));
-                vtop = max(vtop, __shfl_xor_sync(0xffffffffu, vtop, o));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
             }
             if (!(kref > 0.f)) kref = 1.f;
-            const int vexp = vtop ? min(max((int)vtop - 127, -120), 120) : 0;
-            const uint32_t hidden = __ballot_sync(0xffffffffu, blk < 0) & 255u, bad_v = __ballot_sync(0xffffffffu, blk >= 0 && !fine_v) & 255u;
-            const float rk = __shfl_sync(0xffffffffu, ks, w) / kref;
-            const float rv = __shfl_sync(0xffffffffu, fine_v ? vs : 0.f, w) * __uint_as_float((uint32_t)(127 - vexp) << 23);
-            const bool plain_k = rk == 1.f, plain_v = rv == 1.f;
-            const __half2 hk = __float2half2_rn(rk), hv = __float2half2_rn(rv);
+            const int vexp = top ? min(max((int)top - 127, -120), 120) : 0;
+            const uint32_t hidden = __ballot_sync(0xffffffffu, blk < 0) & 255u, bad = __ballot_sync(0xffffffffu, blk >= 0 && !fine) & 255u;
             if (w == 0 && lane == 0) {
-                sh.info[i & 3] = TcaInfo{kref, vexp, hidden, bad_v};
+                TcaInfo& f = sh.info[i & 3];
+                if (is_k) { f.kref = kref; f.hidden = hidden; }
+                else { f.vexp = vexp; f.bad_v = bad; }
                 mbar_arrive(&sh.info_full[i & 3]);
             }
-            // K: key (lane & 7) + 8 a, columns 2 c and 2 c + 1 for the loaded piece c = lane / 8 + 4 j
-            if (i >= 2 && !wait(&sh.k_empty[slot], (i >> 1) - 1)) break;
+            if (i >= 2 && !wait(&empty[slot], (i >> 1) - 1)) break;
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
+            for (int g = 0; g < 2; ++g) {
+                const float own = __shfl_sync(0xffffffffu, sc, w + g);
+                // K over the step's largest scale; V over a power of two, a scale that is not finite as 0
+                const float r = is_k ? own / kref : fabsf(own) <= 3.402823466e38f ? own * __uint_as_float((uint32_t)(127 - vexp) << 23) : 0.f;
+                const bool plain = r == 1.f;
+                const __half2 hr = __float2half2_rn(r);
+                if (is_k) {
 #pragma unroll
-                for (int j = 0; j < KL; ++j) {
-                    const uint32_t x[4] = {kb[a][j].x ^ 0x80808080u, kb[a][j].y ^ 0x80808080u, kb[a][j].z ^ 0x80808080u, kb[a][j].w ^ 0x80808080u};
-                    uint32_t o[8];
+                    for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        o[2 * k] = scaled(__byte_perm(x[k], 0x64646464u, 0x4140), plain_k, hk);
-                        o[2 * k + 1] = scaled(__byte_perm(x[k], 0x64646464u, 0x4342), plain_k, hk);
+                        for (int j = 0; j < KL; ++j) {
+                            const uint4 q = raw[g][a * KL + j];
+                            const uint32_t x[4] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u, q.z ^ 0x80808080u, q.w ^ 0x80808080u};
+                            uint32_t o[8];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                o[2 * k] = scaled(__byte_perm(x[k], 0x64646464u, 0x4140), plain, hr);
+                                o[2 * k + 1] = scaled(__byte_perm(x[k], 0x64646464u, 0x4342), plain, hr);
+                            }
+                            uint8_t* d = sk + slot * KB + (2 * (w + g) + a) * (CG * 128) + 2 * ((lane >> 3) + 4 * j) * 128 + (lane & 7) * 16;
+                            *reinterpret_cast<uint4*>(d) = make_uint4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<uint4*>(d + 128) = make_uint4(o[4], o[5], o[6], o[7]);
+                        }
+                } else {
+                    // transposed: eight keys of one dim are 16 bytes; the lane's four dims in an order that spreads the banks
+                    const uint32_t* q = reinterpret_cast<const uint32_t*>(&raw[g][0]);
+#pragma unroll
+                    for (int v = 0; v < VG; ++v) {
+                        uint32_t o[4][4];                         // [dim slot][pair of keys]
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t x = q[8 * v + 2 * k] ^ 0x80808080u, y = q[8 * v + 2 * k + 1] ^ 0x80808080u;
+                            const uint32_t u0 = __byte_perm(x, y, sel0), u1 = __byte_perm(x, y, sel1);
+                            o[0][k] = scaled(__byte_perm(u0, 0x64646464u, 0x4140), plain, hr);
+                            o[1][k] = scaled(__byte_perm(u0, 0x64646464u, 0x4342), plain, hr);
+                            o[2][k] = scaled(__byte_perm(u1, 0x64646464u, 0x4140), plain, hr);
+                            o[3][k] = scaled(__byte_perm(u1, 0x64646464u, 0x4342), plain, hr);
+                        }
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) {
+                            const int dim = 4 * vd + ((d + rot) & 3);
+                            *reinterpret_cast<uint4*>(sv + slot * KB + (dim >> 3) * (kTcaKeys / 8 * 128) + (2 * (w + g) + vg + v) * 128 + (dim & 7) * 16) = make_uint4(o[d][0], o[d][1], o[d][2], o[d][3]);
+                        }
                     }
-                    uint8_t* d = sk + slot * KB + (2 * w + a) * (CG * 128) + 2 * ((lane >> 3) + 4 * j) * 128 + (lane & 7) * 16;
-                    *reinterpret_cast<uint4*>(d) = make_uint4(o[0], o[1], o[2], o[3]);
-                    *reinterpret_cast<uint4*>(d + 128) = make_uint4(o[4], o[5], o[6], o[7]);
-                }
-            proxy_fence_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.k_full[slot]);
-            // V transposed: eight keys of one dim are 16 bytes; the lane's four dims in an order that spreads the banks
-            if (i >= 2 && !wait(&sh.v_empty[slot], (i >> 1) - 1)) break;
-#pragma unroll
-            for (int g = 0; g < VG; ++g) {
-                uint32_t o[4][4];                                 // [dim slot][pair of keys]
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t x = vb[g][2 * k] ^ 0x80808080u, y = vb[g][2 * k + 1] ^ 0x80808080u;
-                    const uint32_t u = __byte_perm(x, y, sel0), v = __byte_perm(x, y, sel1);
-                    o[0][k] = scaled(__byte_perm(u, 0x64646464u, 0x4140), plain_v, hv);
-                    o[1][k] = scaled(__byte_perm(u, 0x64646464u, 0x4342), plain_v, hv);
-                    o[2][k] = scaled(__byte_perm(v, 0x64646464u, 0x4140), plain_v, hv);
-                    o[3][k] = scaled(__byte_perm(v, 0x64646464u, 0x4342), plain_v, hv);
-                }
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const int dim = 4 * vd + ((d + rot) & 3);
-                    *reinterpret_cast<uint4*>(sv + slot * KB + (dim >> 3) * (kTcaKeys / 8 * 128) + (2 * w + vg + g) * 128 + (dim & 7) * 16) = make_uint4(o[d][0], o[d][1], o[d][2], o[d][3]);
                 }
             }
             proxy_fence_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.v_full[slot]);
-            if (i + 1 < n) load(kt0 + i + 1);
+            if (lane == 0) mbar_arrive(&full[slot]);
+            if (i + 1 < n) load(kt0 + i + 1, blk1);
+            blk = blk1; blk1 = blk2; sc = sc1;
         }
     } else if (warp == 16) {
         // ------------------------------------------------ products
@@ -376,19 +390,20 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
             const int a = z_lo - key0, b = z - key0;
             const bool edge = __any_sync(0xffffffffu, a >= 0 || b < kTcaKeys - 1) || info.hidden;
             auto seen = [&](int col) { return col <= b && col > a && !(info.hidden >> (col >> 4) & 1); };
-            float top = -INFINITY;
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};           // four chains
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 float s[32];
                 tc_ld32(s_at + 32 * c, s);
                 if (edge) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) top = seen(32 * c + k) ? fmaxf(top, s[k]) : top;
+                    for (int k = 0; k < 32; ++k) tops[k & 3] = seen(32 * c + k) ? fmaxf(tops[k & 3], s[k]) : tops[k & 3];
                 } else {
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) top = fmaxf(top, fmaxf(s[k], s[k + 1]));
+                    for (int k = 0; k < 32; k += 2) tops[k >> 1 & 3] = fmaxf(tops[k >> 1 & 3], fmaxf(s[k], s[k + 1]));
                 }
             }
+            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             top = top == -INFINITY ? top : top * f;
             const bool grows = top > m + kAttnSlack, scale_grows = info.vexp > vrun + kTcaScaleSlack;
             if (__any_sync(0xffffffffu, grows) || scale_grows) {
@@ -416,26 +431,30 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                 m = m_new;
             }
             const float m_safe = m == -INFINITY ? 0.f : m, shift = kTcaLift + (float)max(info.vexp - vrun, -100) - m_safe;
-            float sum = 0.f;
+            float sums[4] = {0.f, 0.f, 0.f, 0.f};
+            auto weights = [&](auto masked) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float s[32];
-                tc_ld32(s_at + 32 * c, s);
-                uint32_t u[16];
+                for (int c = 0; c < 4; ++c) {
+                    float s[32];
+                    tc_ld32(s_at + 32 * c, s);
+                    uint32_t u[16];
 #pragma unroll
-                for (int k = 0; k < 32; k += 2) {
-                    float e0 = ex2(fmaf(s[k], f, shift)), e1 = ex2(fmaf(s[k + 1], f, shift));
-                    if (edge) {
-                        e0 = seen(32 * c + k) ? e0 : 0.f;
-                        e1 = seen(32 * c + k + 1) ? e1 : 0.f;
+                    for (int k = 0; k < 32; k += 2) {
+                        float e0 = ex2(fmaf(s[k], f, shift)), e1 = ex2(fmaf(s[k + 1], f, shift));
+                        if constexpr (decltype(masked)::value) {
+                            e0 = seen(32 * c + k) ? e0 : 0.f;
+                            e1 = seen(32 * c + k + 1) ? e1 : 0.f;
+                        }
+                        sums[k & 2] += e0;
+                        sums[(k & 2) + 1] += e1;
+                        u[k >> 1] = pack_half2(e0, e1);
                     }
-                    sum += e0;
-                    sum += e1;
-                    u[k >> 1] = pack_half2(e0, e1);
+                    tc_st16(s_at + 16 * c, u);                  // over scores that were read
                 }
-                tc_st16(s_at + 16 * c, u);                      // over scores that were read
-            }
-            l = fmaf(sum, ex2((float)-max(info.vexp - vrun, -100)), l);
+            };
+            if (edge) weights(std::true_type());
+            else weights(std::false_type());
+            l = fmaf((sums[0] + sums[1]) + (sums[2] + sums[3]), ex2((float)-max(info.vexp - vrun, -100)), l);
             if (info.bad_v)
                 for (int g = 0; g < 8; ++g)                     // a V scale that is not finite: NaN for the rows that see its keys
                     if (info.bad_v >> g & 1 && max(16 * g, a + 1) <= min(16 * g + 15, b)) l = __int_as_float(0x7fc00000);
