@@ -122,6 +122,25 @@ __device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+// Sixteen columns, not waited for; tc_wait16 names the registers, so nothing that uses them moves in front of it.
+__device__ __forceinline__ void tc_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tc_wait16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tc_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Four biased codes -> two pairs of fp16, times r where the group has a factor.
@@ -390,19 +409,26 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
             const int a = z_lo - key0, b = z - key0;
             const bool edge = __any_sync(0xffffffffu, a >= 0 || b < kTcaKeys - 1) || info.hidden;
             auto seen = [&](int col) { return col <= b && col > a && !(info.hidden >> (col >> 4) & 1); };
-            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};           // four chains
+            // f(chunk, its sixteen scores), the next chunk on its way meanwhile
+            auto scores = [&](auto f) {
+                uint32_t r[2][16];
+                tc_ld16_nowait(s_at, r[0]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float s[32];
-                tc_ld32(s_at + 32 * c, s);
-                if (edge) {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) tops[k & 3] = seen(32 * c + k) ? fmaxf(tops[k & 3], s[k]) : tops[k & 3];
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 32; k += 2) tops[k >> 1 & 3] = fmaxf(tops[k >> 1 & 3], fmaxf(s[k], s[k + 1]));
+                for (int c = 0; c < 8; ++c) {
+                    tc_wait16(r[c & 1]);
+                    if (c < 7) tc_ld16_nowait(s_at + 16 * (c + 1), r[(c + 1) & 1]);
+                    f(c, r[c & 1]);
                 }
-            }
+            };
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};           // four chains
+            if (edge) scores([&](int c, const uint32_t (&r)[16]) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) tops[k & 3] = seen(16 * c + k) ? fmaxf(tops[k & 3], __uint_as_float(r[k])) : tops[k & 3];
+            });
+            else scores([&](int, const uint32_t (&r)[16]) {
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) tops[k >> 1 & 3] = fmaxf(tops[k >> 1 & 3], fmaxf(__uint_as_float(r[k]), __uint_as_float(r[k + 1])));
+            });
             float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             top = top == -INFINITY ? top : top * f;
             const bool grows = top > m + kAttnSlack, scale_grows = info.vexp > vrun + kTcaScaleSlack;
@@ -431,30 +457,27 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                 m = m_new;
             }
             const float m_safe = m == -INFINITY ? 0.f : m, shift = kTcaLift + (float)max(info.vexp - vrun, -100) - m_safe;
-            float sums[4] = {0.f, 0.f, 0.f, 0.f};
+            f2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};
             auto weights = [&](auto masked) {
+                scores([&](int c, const uint32_t (&r)[16]) {
+                    uint32_t u[8];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float s[32];
-                    tc_ld32(s_at + 32 * c, s);
-                    uint32_t u[16];
-#pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        float e0 = ex2(fmaf(s[k], f, shift)), e1 = ex2(fmaf(s[k + 1], f, shift));
+                    for (int k = 0; k < 16; k += 2) {
+                        const f2 x = ffma2(f2{__uint_as_float(r[k]), __uint_as_float(r[k + 1])}, f2{f, f}, f2{shift, shift});
+                        float e0 = ex2(x.x), e1 = ex2(x.y);
                         if constexpr (decltype(masked)::value) {
-                            e0 = seen(32 * c + k) ? e0 : 0.f;
-                            e1 = seen(32 * c + k + 1) ? e1 : 0.f;
+                            e0 = seen(16 * c + k) ? e0 : 0.f;
+                            e1 = seen(16 * c + k + 1) ? e1 : 0.f;
                         }
-                        sums[k & 2] += e0;
-                        sums[(k & 2) + 1] += e1;
+                        sums[k >> 1 & 1] = fadd2(sums[k >> 1 & 1], f2{e0, e1});
                         u[k >> 1] = pack_half2(e0, e1);
                     }
-                    tc_st16(s_at + 16 * c, u);                  // over scores that were read
-                }
+                    tc_st8(s_at + 8 * c, u);                    // over scores that were read
+                });
             };
             if (edge) weights(std::true_type());
             else weights(std::false_type());
-            l = fmaf((sums[0] + sums[1]) + (sums[2] + sums[3]), ex2((float)-max(info.vexp - vrun, -100)), l);
+            l = fmaf((sums[0].x + sums[0].y) + (sums[1].x + sums[1].y), ex2((float)-max(info.vexp - vrun, -100)), l);
             if (info.bad_v)
                 for (int g = 0; g < 8; ++g)                     // a V scale that is not finite: NaN for the rows that see its keys
                     if (info.bad_v >> g & 1 && max(16 * g, a + 1) <= min(16 * g + 15, b)) l = __int_as_float(0x7fc00000);
