@@ -103,5 +103,19 @@ def test_wrappers_refuse_shapes_types_and_strides():
     for bad in ((k.half(), k, s, s), (k, k[:4], s, s), (k, k.transpose(1, 2), s, s), (k, k, s[:4], s), (k, k, s, s.double())):
         with pytest.raises(ValueError):
             K.KvCache(*bad)
-    with pytest.raises(ValueError, match="k_out"):
-        K.kv_read_q8(None, i, None, None)
+    for args in ((i, None, None), (i, h.double(), None)):
+        with pytest.raises(ValueError, match="k_out"):
+            K._step().kv_read_q8(0, k, 2, 64, *args, 0, None)
+    six = [torch.zeros(6, dtype=torch.int32) for _ in range(12)]
+    with pytest.raises(ValueError, match="block_table"):
+        K.kv_plan(*six, 16)
+    for q, y in ((h, h[:2]), (h[0], h), (h.double(), h)):
+        with pytest.raises(ValueError, match="q|y"):
+            K._step().attn_q8(q, y, i, i, i, 0, k, 64, i, 1, 1.0, 0, 0, None)
+    for q, kk, v in ((None, h, h[:2]), (None, h, h.float()), (h[:2], h, h), (h.float(), h, h)):
+        with pytest.raises(ValueError):
+            K._step().rope_append_q8(q, kk, v, q, i, 0, k, 4, 64, None, None, 0, None)
+    with pytest.raises(ValueError, match="number of arguments"):
+        K._step().sample(h)
+    with pytest.raises(ValueError, match="a tensor expected"):
+        K._step().sample(*[3] * 10)

@@ -32,6 +32,10 @@ def _stream(stream):
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
+def _stream_arg(stream):
+    return stream if stream is None else _stream(stream)
+
+
 def q4_gpu_data_offset(total_blocks: int) -> int:
     """tensor.Q4GPUDataOffset (tensor/quantized.go:196-199)."""
     return (total_blocks * 2 + 15) & ~15
@@ -255,7 +259,7 @@ def describe_plan(fmt: str, n: int, k: int, batch: int = 1, group: int = 128, sm
 
 
 # ---- the decode step around the projections: plan, rotary positions + 8-bit cache, attention, sampling.  Tensors carry
-# shapes, strides and types, so these wrappers check them here; X_F32 / Y_F32 follow from the dtypes.
+# shapes, strides and types, so these wrappers (the frequent ones in host/ztq_py.cc) check them; X_F32 / Y_F32 follow from the dtypes.
 
 ROPE_PAIRS = 128
 ROPE_SCALING = {"none": 0, "linear": 1, "by_turns": 2, "by_dim": 3}
@@ -264,23 +268,9 @@ SAMPLE_MAX_VOCAB = 327680
 
 def _arg(t, dtype, shape, name):
     """Device pointer of a contiguous tensor of this type and shape on the current device."""
-    return _args((dtype, t, shape, name))[0]
-
-
-def _args(*wanted):
-    """Device pointers of (type, tensor, shape, name): contiguous tensors of that type and shape on the current device; 0 for None.
-    One loop with nothing but the checks in it: a step makes dozens of these calls, and they cost more than a small launch."""
-    dev, out = _device(), []
-    for dtype, t, shape, name in wanted:
-        if t is None:
-            out.append(0)
-        elif t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == dev:
-            out.append(t.data_ptr())
-        elif t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
-            raise ValueError(f"{name}: contiguous {dtype} {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}")
-        else:
-            raise ValueError(f"{name}: a tensor on the current CUDA device expected, got one on {t.device}")
-    return out
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous {dtype} {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}")
+    return _here(t, name)
 
 
 def _device():
@@ -303,6 +293,22 @@ def _heads(t, name):
     if len(strides) != 3 or not (f32 or t.dtype is torch.float16) or strides[2] != 1:
         raise ValueError(f"{name}: float16 or float32 [tokens, heads, dim] with contiguous dim expected, got {t.dtype} {tuple(t.shape)}, strides {strides}")
     return _here(t, name), strides[0], strides[1], f32
+
+
+_native = None
+
+
+def _step():
+    """The native entry points of the operators that a step calls many times (host/ztq_py.cc): checks and launch in one call."""
+    global _native
+    if _native is None:
+        _lib.lib()
+        try:
+            from . import _step as module
+        except ImportError as e:
+            raise _lib.KernelLibraryMissing(f"ztensor_b200/_step.so cannot be loaded ({e}): build it with `make -C ztensor_b200/host`") from e
+        _native = module
+    return _native
 
 
 class ZtqKvCache(C.Structure):
@@ -330,6 +336,7 @@ class KvCache:
         self.blocks, self.kv_heads, self.block_size, self.head_dim = blocks, heads, size, dim
         self.desc = ZtqKvCache(_here(k, "k"), _here(v, "v"), k_scale.data_ptr(), v_scale.data_ptr(), k.stride(0) if blocks > 1 else heads * size * dim, blocks, heads, size, dim)
         self.ptr = C.addressof(self.desc)
+        self.codes = k
 
     @classmethod
     def empty(cls, blocks, kv_heads, block_size, head_dim, device="cuda"):
@@ -337,21 +344,11 @@ class KvCache:
         k, v = (torch.empty(blocks, kv_heads, block_size, head_dim, dtype=torch.int8, device=device) for _ in range(2))
         return cls(k, v, *(torch.zeros(blocks, kv_heads, device=device) for _ in range(2)))
 
-    def _on(self):
-        _here(self.tensors[0], "cache")
-        return self.ptr
-
 
 def kv_plan(ctx_len, new_len, block_table, ring, ring_state, ring_state_out, next_len, kv_len, query_start, positions, slots, status, block_size, flags=0, stream=None):
     """The plan of a step: block table, slots, positions and lengths from the sequences' lengths (ztq_kv_plan).
     All int32; next_len may be ctx_len and ring_state_out may be ring_state."""
-    i, n, rows, width, pool = torch.int32, ctx_len.shape[0], slots.shape[0], block_table.shape[-1], ring.shape[0]
-    per_seq, per_row = (n,), (rows,)
-    _lib.check(_lib.lib().ztq_kv_plan(
-        *_args((i, ctx_len, per_seq, "ctx_len"), (i, new_len, per_seq, "new_len"), (i, block_table, (n, width), "block_table"), (i, ring, (pool,), "ring"),
-               (i, ring_state, (2,), "ring_state"), (i, ring_state_out, (2,), "ring_state_out"), (i, next_len, per_seq, "next_len"), (i, kv_len, per_seq, "kv_len"),
-               (i, query_start, (n + 1,), "query_start"), (i, positions, per_row, "positions"), (i, slots, per_row, "slots"), (i, status, per_seq, "status")),
-        n, width, block_size, pool, rows, flags, _stream(stream)), "ztq_kv_plan")
+    _step().kv_plan(ctx_len, new_len, block_table, ring, ring_state, ring_state_out, next_len, kv_len, query_start, positions, slots, status, block_size, flags, _stream_arg(stream))
 
 
 def rope_table(rows, rot_dim, base, first=0, scaling="none", factor=1.0, turns_low=1.0, turns_high=4.0, original_positions=0, magnitude=1.0, out=None, flags=0, stream=None):
@@ -379,34 +376,12 @@ def rope(x, y, table, positions, flags=0, stream=None):
 def rope_append_q8(q, k, v, q_out, slots, cache, table=None, positions=None, flags=0, stream=None):
     """Rotates q [tokens, q_heads, dim] into q_out (both may be None, or q_out may be q) and appends k (rotated), v [tokens, kv_heads, dim] to
     the cache at `slots` (ztq_rope_append_q8).  table None: nothing is rotated.  flags: ROPE_PAIRS, NO_PDL."""
-    kp, kt, kh, xf = _heads(k, "k")
-    vp, vt, vh, vf = _heads(v, "v")
-    n = k.shape[0]
-    if k.shape != (n, cache.kv_heads, cache.head_dim) or v.shape != k.shape or vf != xf:
-        raise ValueError(f"k, v: one type and {(n, cache.kv_heads, cache.head_dim)} expected, got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
-    qp = qo = qt = qh = ot = oh = heads = 0
-    of = False
-    if q is not None:
-        qp, qt, qh, qf = _heads(q, "q")
-        qo, ot, oh, of = _heads(q_out, "q_out")
-        heads = q.shape[1]
-        if qf != xf or q.shape[0] != n or q.shape[2] != cache.head_dim or q_out.shape != q.shape:
-            raise ValueError(f"q, q_out: {n} rows of heads of {cache.head_dim} and the type of k expected, got {q.dtype} {tuple(q.shape)} and {tuple(q_out.shape)}")
-    rows, half = table.shape[:2] if table is not None else (0, 0)
-    i = torch.int32
-    tp, pp, sp = _args((torch.float32, table, (rows, half, 2), "table"), (i, positions if table is not None else None, (n,), "positions"), (i, slots, (n,), "slots"))
-    _lib.check(_lib.lib().ztq_rope_append_q8(qp, kp, vp, qo, qt, qh, kt, kh, vt, vh, ot, oh, n, heads, tp, rows, 2 * half, pp, sp, cache._on(), flags | (X_F32 if xf else 0) | (Y_F32 if of else 0), _stream(stream)), "ztq_rope_append_q8")
+    _step().rope_append_q8(q, k, v, q_out, slots, cache.ptr, cache.codes, cache.kv_heads, cache.head_dim, table, positions, flags, _stream_arg(stream))
 
 
 def kv_read_q8(cache, slots, k_out, v_out, flags=0, stream=None):
     """The cache's rows at `slots`, dequantized into k_out and v_out [tokens, kv_heads, dim] (either may be None) (ztq_kv_read_q8)."""
-    out = k_out if k_out is not None else v_out
-    if out is None or (out.dtype is not torch.float16 and out.dtype is not torch.float32):
-        raise ValueError("k_out, v_out: at least one float16 or float32 tensor expected")
-    n = slots.shape[0]
-    shape = (n, cache.kv_heads, cache.head_dim)
-    sp, kp, vp = _args((torch.int32, slots, (n,), "slots"), (out.dtype, k_out, shape, "k_out"), (out.dtype, v_out, shape, "v_out"))
-    _lib.check(_lib.lib().ztq_kv_read_q8(cache._on(), sp, n, kp, vp, flags | (Y_F32 if out.dtype is torch.float32 else 0), _stream(stream)), "ztq_kv_read_q8")
+    _step().kv_read_q8(cache.ptr, cache.codes, cache.kv_heads, cache.head_dim, slots, k_out, v_out, flags, _stream_arg(stream))
 
 
 def attn_q8_workspace_bytes(tokens, sequences, max_new, q_heads, kv_heads, head_dim) -> int:
@@ -415,25 +390,9 @@ def attn_q8_workspace_bytes(tokens, sequences, max_new, q_heads, kv_heads, head_
 
 def attn_q8(q, y, query_start, kv_len, block_table, cache, workspace, max_new, scale, window=0, flags=0, stream=None):
     """Causal attention of q [tokens, q_heads, dim] over the cache into y (ztq_attn_q8); window 0: all earlier positions."""
-    qp, qt, qh, xf = _heads(q, "q")
-    yp, yt, yh, yf = _heads(y, "y")
-    n, heads, dim = q.shape
-    seqs = kv_len.shape[0]
-    if y.shape != q.shape or dim != cache.head_dim:
-        raise ValueError(f"q, y: one shape and heads of {cache.head_dim} expected, got {tuple(q.shape)} and {tuple(y.shape)}")
-    i, width = torch.int32, block_table.shape[-1]
-    sp, lp, bp = _args((i, query_start, (seqs + 1,), "query_start"), (i, kv_len, (seqs,), "kv_len"), (i, block_table, (seqs, width), "block_table"))
-    _lib.check(_lib.lib().ztq_attn_q8(qp, yp, qt, qh, yt, yh, n, heads, sp, lp, bp, seqs, width, max_new, window, C.c_uint.from_buffer(C.c_float(scale)).value, cache._on(),
-                                      _here(workspace, "workspace"), workspace.nbytes, flags | (X_F32 if xf else 0) | (Y_F32 if yf else 0), _stream(stream)), "ztq_attn_q8")
+    _step().attn_q8(q, y, query_start, kv_len, block_table, cache.ptr, cache.codes, cache.head_dim, workspace, max_new, scale, window, flags, _stream_arg(stream))
 
 
 def sample(logits, uniform, token, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None, flags=0, stream=None):
     """One token per row of logits [rows, vocab] from `uniform` [rows] in [0, 1) (ztq_sample)."""
-    if logits.dim() != 2 or (logits.dtype is not torch.float16 and logits.dtype is not torch.float32) or (logits.stride(1) != 1 and logits.shape[1] > 1):
-        raise ValueError(f"logits: float16 or float32 [rows, vocab] with contiguous rows expected, got {logits.dtype} {tuple(logits.shape)}, strides {logits.stride()}")
-    n, vocab = logits.shape
-    f, i, rows = torch.float32, torch.int32, (n,)
-    _lib.check(_lib.lib().ztq_sample(
-        _here(logits, "logits"), logits.stride(0) if n > 1 else 0, n, vocab,
-        *_args((f, temperature, rows, "temperature"), (i, top_k, rows, "top_k"), (f, top_p, rows, "top_p"), (f, min_p, rows, "min_p"), (f, uniform, rows, "uniform"), (i, token, rows, "token"),
-               (f, logprob, rows, "logprob")), flags | (X_F32 if logits.dtype is torch.float32 else 0), _stream(stream)), "ztq_sample")
+    _step().sample(logits, uniform, token, logprob, temperature, top_k, top_p, min_p, flags, _stream_arg(stream))
