@@ -6,10 +6,10 @@
 // T = 0 takes the first of the order.
 //
 // No row is sorted.  A cut of the ordered row is (key, m): everything above the key and the first m tokens equal to it.
-// Keys are the logits' bits mapped to unsigned order.  A cut is found in two steps, by counts for k and by mass for p: a
+// Keys are the logits' bits mapped to unsigned order.  A cut is found in steps, by counts for k and by mass for p: a
 // histogram over log2(w) in 16ths (on the bits of the logits most of a row would fall into a few dozen bins, whose atomics
-// serialize), then the few keys of the bin that holds the cut compared with one another; where that bin holds more than
-// 512 keys, a radix selection on its keys.
+// serialize), if its bin holds more than a few keys a second one over 1024ths of that bin, then the keys that are left
+// compared with one another; where they are still more than 511 (ties, or a bin without a lower end), a radix selection.
 // Masses are 64-bit fixed point, w = W / 2^44: integer sums do not depend on the order in which atomics or CTAs add them, so
 // the same row gives the same token on any launch, and W is computed in 64 bits, because an error of an fp32 exp moves all
 // borders behind a likely token: over a large vocabulary u would meet a moved border once in a few hundred rows.
@@ -41,7 +41,9 @@ constexpr int kSampleMaxSlice = 40960;             // keys of one CTA (fp32: 160
 constexpr int kSampleMaxSegs = kSampleMaxSlice / kSampleSeg;
 constexpr int kSampleFrac = 44;
 constexpr int kSampleCand = kSampleThreads;        // keys of a bin that are compared directly, of all ranks
+constexpr int kSampleFew = 64;                     // below this they are compared at once, else the bin is divided further first
 constexpr int kSampleList = 192;                   // tokens that are ranked directly
+constexpr int kSampleKeep = 2048;                  // keys of a slice that are kept apart, so that later passes need not look at all
 constexpr int kSampleGroups = 4;                   // groups of lanes of a warp whose maxima are kept
 
 struct SampleParams {
@@ -103,6 +105,7 @@ struct SampleShared {
     uint32_t found_bin, cands, found_key;
     uint32_t cand[kSampleCand], all[kSampleCand];
     unsigned long long all_mass[kSampleCand];
+    uint32_t list[kSampleKeep];
     unsigned long long found_above, found_total;
 };
 
@@ -279,6 +282,10 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
         const float d = (l_max - l) * c16;
         return l == l_max ? kSampleBins - 1 : d < (float)(kSampleBins - 1) ? kSampleBins - 1 - (int)d : 0;
     };
+    auto fine = [&](float l) {                             // its place within a bin other than 0
+        const float d = l == l_max ? 0.f : (l_max - l) * c16;
+        return kSampleBins - 1 - (int)((d - floorf(d)) * (float)kSampleBins);
+    };
     const double l_min = floor_p > 0.f ? (double)l_max + (double)temp * log((double)floor_p) : -1e300;
     const uint32_t key_min = floor_p > 0.f ? Key::least(l_min) : 0;
     const bool any = best > Key::of(F32 ? 0xff800000u : 0xfc00u);         // something to draw
@@ -298,6 +305,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
         if (tid < n_g) {
             const uint32_t v = sh.all[tid];
             int over = 0;
+#pragma unroll 8
             for (int j = 0; j < n_g; ++j) over += sh.all[j] > v || (sh.all[j] == v && j < tid);
             if (over == k - 1) sh.found_key = v;
         }
@@ -327,6 +335,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
             p.logprob[row] = greedy ? 0.f : (float)((weight.top_inf ? 0.0 : ((double)l - weight.top) / (double)temp) - log((double)total / (double)(1ull << kSampleFrac)));
     };
 
+    int n_list = -1;                                       // keys in sh.list, if they are all that matters
     // ---- few tokens reach the bound: rank 0 takes them all
     if (any && low > 0) {
         const bool whole = k <= 0 && share < 1.f;          // top-p of everything: its mass is wanted too
@@ -339,6 +348,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
                 if (key >= low) {
                     const uint32_t at = atomicAdd(&sh.cands, 1u);
                     if (at < kSampleList) { sh.cand[at] = key; sh.index[at] = (uint32_t)(lo + j); }
+                    if (at < kSampleKeep) sh.list[at] = key;
                 }
             }
             if (whole) each_weight(s, [](uint32_t) { return true; }, [&](uint32_t, float, unsigned long long w) { sum += w; });
@@ -410,6 +420,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
             cluster.sync();                                // the lists have been read
             return;
         }
+        if (k > 0 && sh.cands <= kSampleKeep) n_list = (int)sh.cands;
         cluster.sync();                                    // the counters and sums have been read
     }
 
@@ -471,13 +482,20 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
         constexpr bool MASSES = decltype(masses)::value;
         const bool first = rank == 0 && tid == 0 && floor_mass != 0;      // the one who adds the floor's mass
         unsigned long long rest = 0;
-        if constexpr (MASSES) {
-            for (int s = warp; s < segs; s += warps)
-                each_weight(s, [&](uint32_t key) { return key > floor; }, [&](uint32_t key, float l, unsigned long long w) {
-                    if (key < least) rest += w;
-                    else if (w) add_mass(coarse(l), w);
-                });
-        } else each([&](uint32_t key) { if (key >= least) atomicAdd(&sh.hist[buffer][0][coarse(Key::value(key))], 1u); });
+        int kept = n_list;                                // keys of sh.list to go through instead of all; -1: all
+        auto each_kept = [&](auto f) {
+            if (kept < 0) each(f);
+            else for (int i = tid; i < kept; i += kSampleThreads) f(sh.list[i]);
+        };
+        each_kept([&](uint32_t key) {
+            if constexpr (MASSES) {
+                if (key <= floor) return;
+                const float l = Key::value(key);
+                const unsigned long long w = weight(l);
+                if (key < least) rest += w;
+                else if (w) add_mass(coarse(l), w);
+            } else if (key >= least) atomicAdd(&sh.hist[buffer][0][coarse(Key::value(key))], 1u);
+        });
         if constexpr (MASSES) {                           // (its high digit takes part of 32 bits: at most 16 such adds)
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
@@ -488,56 +506,87 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
         want = select(want, 0, MASSES);
         unsigned long long above = sh.found_above;
         const int bin = (int)sh.found_bin;
-        auto inside = [&](uint32_t key) { return key >= least && (key > floor || !floor) && coarse(Key::value(key)) == bin; };
-        each([&](uint32_t key) {
-            if (inside(key)) {
-                const uint32_t at = atomicAdd(&sh.cands, 1u);
-                if (at < kSampleCand) sh.cand[at] = key;
-            }
-        });
-        cluster.sync();
-        uint32_t total = 0;
-        for (int r = 0; r < ranks; ++r) {
-            const uint32_t c = *cluster.map_shared_rank(&sh.cands, r);
-            const uint32_t* from = cluster.map_shared_rank(&sh.cand[0], r);
-            if (total + c <= kSampleCand - 1)
-                for (uint32_t i = tid; i < c; i += kSampleThreads) sh.all[total + i] = from[i];
-            total += c;
-        }
-        const bool with_floor = floor_mass != 0 && coarse(Key::value(floor)) == bin;
-        if (total <= kSampleCand - 1) {
-            if (with_floor && tid == 0) sh.all[total] = floor;
-            if (with_floor) ++total;
-            __syncthreads();
-            uint32_t key = 0;
-            if (tid < total) {
-                key = sh.all[tid];
-                if constexpr (MASSES) sh.all_mass[tid] = with_floor && tid == total - 1 ? floor_mass : weight(Key::value(key));
-            }
-            __syncthreads();
-            if (tid < total) {
-                unsigned long long over = above, same = 0;
-                for (uint32_t j = 0; j < total; ++j) {
-                    const uint32_t other = sh.all[j];
-                    const unsigned long long w = MASSES ? sh.all_mass[j] : 1ull;
-                    over += other > key ? w : 0ull;
-                    same += other == key ? w : 0ull;
+        // keys of the bin; of one 1024th of it in the second round
+        int fine_bin = -1;
+        auto inside = [&](uint32_t key) {
+            if (key < least || (key <= floor && floor)) return false;
+            const float l = Key::value(key);
+            return coarse(l) == bin && (fine_bin < 0 || fine(l) == fine_bin);
+        };
+        auto floor_inside = [&]() {
+            const float l = Key::value(floor);
+            return floor_mass != 0 && coarse(l) == bin && (fine_bin < 0 || fine(l) == fine_bin);
+        };
+        for (int round = 0;; ++round) {
+            const bool fills = kept < 0;                      // the list is free: it takes the bin's keys
+            each_kept([&](uint32_t key) {
+                if (inside(key)) {
+                    const uint32_t at = atomicAdd(&sh.cands, 1u);
+                    if (at < kSampleCand) sh.cand[at] = key;
+                    if (fills && at < kSampleKeep) sh.list[at] = key;
                 }
-                if ((double)over < want && (double)(over + same) >= want) {
-                    sh.found_key = key;
-                    sh.found_above = over;
+            });
+            cluster.sync();
+            if (fills && sh.cands <= kSampleKeep) kept = (int)sh.cands;
+            uint32_t total = 0;
+            for (int r = 0; r < ranks; ++r) total += min(*cluster.map_shared_rank(&sh.cands, r), (uint32_t)kSampleCand);
+            if (total < (round ? kSampleCand : kSampleFew)) {
+                uint32_t at = 0;
+                for (int r = 0; r < ranks; ++r) {
+                    const uint32_t c = *cluster.map_shared_rank(&sh.cands, r);
+                    if (tid >= at && tid < at + c) sh.all[tid] = cluster.map_shared_rank(&sh.cand[0], r)[tid - at];
+                    at += c;
                 }
+                const bool with_floor = floor_inside();
+                if (with_floor && tid == total) sh.all[total] = floor;
+                if (with_floor) ++total;
+                __syncthreads();
+                uint32_t key = 0;
+                if (tid < total) {
+                    key = sh.all[tid];
+                    if constexpr (MASSES) sh.all_mass[tid] = with_floor && tid == total - 1 ? floor_mass : weight(Key::value(key));
+                }
+                __syncthreads();
+                if (tid < total) {
+                    unsigned long long over = above, same = 0;
+#pragma unroll 8
+                    for (uint32_t j = 0; j < total; ++j) {
+                        const uint32_t other = sh.all[j];
+                        const unsigned long long w = MASSES ? sh.all_mass[j] : 1ull;
+                        if (other > key) over += w;
+                        if (other == key) same += w;
+                    }
+                    if ((double)over < want && (double)(over + same) >= want) {
+                        sh.found_key = key;
+                        sh.found_above = over;
+                    }
+                }
+                cluster.sync();                               // the lists have been read, the cut is there
+                return sh.found_key;
             }
-            cluster.sync();                               // the lists have been read, the cut is there
-            return sh.found_key;
+            cluster.sync();                                   // the counters have been read
+            if (round == 1 || bin == 0) break;                // bin 0 has no lower end
+            if (tid == 0) sh.cands = 0;
+            each_kept([&](uint32_t key) {
+                if (!inside(key)) return;
+                const float l = Key::value(key);
+                if constexpr (MASSES) {
+                    const unsigned long long w = weight(l);
+                    if (w) add_mass(fine(l), w);
+                } else atomicAdd(&sh.hist[buffer][0][fine(l)], 1u);
+            });
+            if (first && floor_inside()) add_mass(fine(Key::value(floor)), floor_mass);
+            select(want, above, MASSES);
+            above = sh.found_above;
+            fine_bin = (int)sh.found_bin;
         }
-        cluster.sync();                                   // the counters have been read
+        const bool with_floor = floor_inside();
         uint32_t prefix = 0;
         for (int pass = 0; pass < Key::kPasses; ++pass) {
             const int shift = Key::shift(pass), up = Key::bits(pass);
             const uint32_t mask = (1u << up) - 1;
             auto matches = [&](uint32_t key) { return pass == 0 || (key >> shift) >> up == prefix; };
-            each([&](uint32_t key) {
+            each_kept([&](uint32_t key) {
                 if (!inside(key) || !matches(key)) return;
                 if constexpr (MASSES) {
                     const unsigned long long w = weight(Key::value(key));
