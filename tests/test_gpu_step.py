@@ -346,6 +346,23 @@ def test_attn_long(lens, heads, group, dim):
     attn_run(lens, heads, group, 64, dim, seed=len(lens))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 3, 50])
+def test_attn_scales_of_any_kind(new, dim):
+    """Scales that are no powers of two, far apart, zero and negative: the append writes none of these, other writers may."""
+    lens = [(300, new), (50 + new, new)]
+    rng = U.seeded(13)
+    cache, table, start, kv_len, q, y = attn_case(rng, lens, 2, 4, 16, dim, torch.float16)
+    for t in cache.tensors[2:]:
+        s = rng.uniform(0.5, 1.5, t.shape) * np.exp2(rng.integers(-16, -4, t.shape)) * rng.choice([1, 1, 1, -1, 0], t.shape)
+        t.copy_(dev(s.astype(np.float32)))
+    ws = torch.empty(K.attn_q8_workspace_bytes(q.shape[0], 2, new, 8, 2, dim), dtype=torch.uint8, device=DEV)
+    for scale in (0.1, -0.1, 0.0):
+        K.attn_q8(q, y, start, kv_len, table, cache, ws, new, scale)
+        attn_check(lens, cache, table, start, q, y, scale, 0, False)
+    no_error()
+
+
 @pytest.mark.parametrize("new", [1, 3, 40])
 def test_attn_rows_that_see_nothing_are_zero(new):
     """More rows than cached tokens: the first rows stand before position 0."""
@@ -624,6 +641,22 @@ def test_decode_steps_together(captured):
         used = [t for b in range(5) for t in s.table[b, :-(-int(s.ctx[b]) // 16)].tolist()]
         free = [int(s.ring[(int(s.state[0]) + i) % 24]) for i in range(int(s.state[1]))]
         assert sorted(used + free) == list(range(24))
+    no_error()
+
+
+def test_calls_without_rows_do_nothing():
+    cache = random_cache(U.seeded(14), 4, 2, 16, 64)
+    before = [t.clone() for t in cache.tensors]
+    i = lambda *n: torch.zeros(*n, dtype=torch.int32, device=DEV)  # noqa: E731
+    h = lambda heads: torch.zeros(0, heads, 64, dtype=torch.float16, device=DEV)  # noqa: E731
+    table = K.rope_table(4, 64, 10000.0)
+    K.rope(h(3), h(3), table, i(0))
+    K.rope_append_q8(h(8), h(2), h(2), h(8), i(0), cache, table, i(0))
+    K.kv_read_q8(cache, i(0), h(2), h(2))
+    K.attn_q8(h(8), h(8), i(3), i(2), i(2, 1), cache, torch.empty(K.attn_q8_workspace_bytes(0, 2, 1, 8, 2, 64), dtype=torch.uint8, device=DEV), 1, 0.1)
+    K.sample(torch.zeros(0, 9, device=DEV), torch.zeros(0, device=DEV), i(0))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, cache.tensors))
     no_error()
 
 

@@ -6,12 +6,11 @@
 //   P_t = 2^(S_t f - m + lift) as fp16, over the columns of S_t
 //   O_t += P_t V    (P_t from TMEM, V^T from shared memory; D columns)
 // The codes become fp16 operands (exactly) on the way into shared memory, once per step for both tiles: a step's 64 KB of
-// operands cost what a quarter of the exponentials costs.  Within a step K codes are multiplied by their block's scale over
-// the step's largest, V codes by theirs over a power of two near the step's largest, so that one factor per step remains
-// (exact for the powers of two that the append writes; other scales are rounded to fp16).
+// operands cost what a quarter of the exponentials costs.  The scales stay out of the operands: sixteen keys are a chunk of
+// scores in the softmax, whose exponent's factor takes sk and whose weights take sv over a running power of two.
 //
-// Roles of the 17 warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread is a row: TMEM lane), 8-11 K codes -> operand, 12-15
-// V codes (32 keys of a step each, loaded one step ahead, their blocks and scales two), 16 issues the products.  The two tiles alternate: while one is in its softmax
+// Roles of the warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread is a row: TMEM lane), then kTcaConv for K codes ->
+// operand and kTcaConv for V (loaded one step ahead, their blocks and scales two), the last issues the products.  The two tiles alternate: while one is in its softmax
 // the tensor cores work for the other.  The running maximum moves only when a score exceeds it by more than kAttnSlack
 // (then the row's O is rescaled in TMEM), as does the reference of the V scales.
 // Operands stand in the canonical K-major layout without swizzle: core matrices of 8 rows x 16 bytes, 128 bytes apart along
@@ -32,14 +31,17 @@
 namespace ztq {
 
 constexpr int kTcaRows = 256, kTcaKeys = 128;
-constexpr int kTcaThreads = 17 * 32;
-constexpr float kTcaLift = 5.f;                 // with kAttnSlack and kTcaScaleSlack: P < 2^15
+constexpr int kTcaConv = 4;                      // warps that convert K, and as many V (two each would leave every thread 128 registers: 596 against 589 us for a chunk of 4096 over 8192)
+constexpr int kTcaGroups = 8 / kTcaConv;         // groups of 16 keys that each of them takes
+constexpr int kTcaMma = 8 + 2 * kTcaConv;
+constexpr int kTcaThreads = 32 * (kTcaMma + 1);
+constexpr float kTcaLift = 4.f;                 // with kAttnSlack, kTcaScaleSlack and the scales' significands below 2: P < 2^15
 constexpr int kTcaScaleSlack = 2;
 
-struct TcaInfo {                                // one step's factors
-    float kref;                                 // scores: S * kref
-    int vexp;                                   // V operand = value / 2^vexp
-    uint32_t hidden, bad_v;                     // groups of 16 keys without a block; with a V scale that is not finite
+struct __align__(16) TcaInfo {                  // one step's factors, by groups of 16 keys
+    float ks[8], vs[8];                         // |K scale|; V scale / 2^vexp, 0 where it is not finite
+    int vexp;
+    uint32_t hidden, bad_v;                     // groups without a block; groups whose V scale is not finite
 };
 
 struct TcaShared {
@@ -132,9 +134,7 @@ __device__ __forceinline__ void tc_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]
 __device__ __forceinline__ void tc_wait16(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
 }
 __device__ __forceinline__ void tc_st8(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
@@ -143,13 +143,7 @@ __device__ __forceinline__ void tc_st8(uint32_t taddr, const uint32_t (&r)[8]) {
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Four biased codes -> two pairs of fp16, times r where the group has a factor.
-__device__ __forceinline__ uint32_t scaled(uint32_t x, bool plain, __half2 r) {
-    const uint32_t u = unbias(x);
-    if (plain) return u;
-    const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&u), r);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
+__device__ __forceinline__ uint32_t turned(uint32_t x, bool plus) { return plus ? unbias(x) : unbias(x) ^ 0x80008000u; }
 
 template <int D>
 __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams tp) {
@@ -179,14 +173,14 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.k_full[i], 4); mbar_init(&sh.k_empty[i], 1);
-            mbar_init(&sh.v_full[i], 4); mbar_init(&sh.v_empty[i], 1);
+            mbar_init(&sh.k_full[i], kTcaConv); mbar_init(&sh.k_empty[i], 1);
+            mbar_init(&sh.v_full[i], kTcaConv); mbar_init(&sh.v_empty[i], 1);
             mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 128); mbar_init(&sh.o_full[i], 1);
         }
         for (int i = 0; i < 4; ++i) mbar_init(&sh.info_full[i], 2);
         mbar_fence_init();
     }
-    if (warp == 16) {
+    if (warp == kTcaMma) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -223,10 +217,10 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
         return ok;
     };
 
-    if (warp >= 8 && warp < 16) {
-        // ------------------------------------------------ codes -> operands: warps 8-11 K, 12-15 V, 32 keys each
-        const bool is_k = warp < 12;
-        const int w = (warp & 3) * 2;                             // first of the warp's two groups of 16 keys
+    if (warp >= 8 && warp < kTcaMma) {
+        // ------------------------------------------------ codes -> operands: one half of the warps K, the other V
+        const bool is_k = warp < 8 + kTcaConv;
+        const int w = (warp - 8) % kTcaConv * kTcaGroups;         // first of the warp's groups of 16 keys
         const int* table = p.block_table + (long long)it.b * p.width;
         constexpr int KL = D / 64, LR = D / 4, VG = LR / 16;      // 16-byte loads per key and lane; lanes per row of V, key groups per lane
         const int vg = lane / LR, vd = lane % LR;                 // V: first key group, word of four dims
@@ -251,10 +245,10 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
             return blk;
         };
         auto scale_of = [&](int blk) { return blk >= 0 ? scales[(long long)blk * p.kv_heads + it.h] : 0.f; };
-        uint4 raw[2][2 * KL];                                     // 16 keys' codes of this lane, twice
+        uint4 raw[kTcaGroups][2 * KL];                            // 16 keys' codes of this lane, for every group
         auto load = [&](int kt, int blks) {
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
+            for (int g = 0; g < kTcaGroups; ++g) {
                 const int own = __shfl_sync(0xffffffffu, blks, w + g);
                 const int at = (kt * kTcaKeys + 16 * (w + g)) & ((1 << p.shift) - 1);
                 const int8_t* src = codes + max(own, 0) * p.block_stride + (((long long)it.h << p.shift) + at) * D;
@@ -284,30 +278,28 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
             const float sc1 = scale_of(blk1);
             // factors of the step
             const bool fine = fabsf(sc) <= 3.402823466e38f;
-            float kref = fine ? fabsf(sc) : 0.f;
-            uint32_t top = fine ? __float_as_uint(fabsf(sc)) >> 23 : 0u;
+            TcaInfo& f = sh.info[i & 3];
+            if (warp == 8) {
+                if (lane < 8) f.ks[lane] = fabsf(sc);
+                const uint32_t hidden = __ballot_sync(0xffffffffu, blk < 0) & 255u;
+                if (lane == 0) f.hidden = hidden;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.info_full[i & 3]);
+            } else if (warp == 8 + kTcaConv) {
+                uint32_t top = fine ? __float_as_uint(fabsf(sc)) >> 23 : 0u;
 #pragma unroll
-            for (int o = 1; o < 8; o <<= 1) {
-                kref = fmaxf(kref, __shfl_xor_sync(0xffffffffu, kref, o));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            }
-            if (!(kref > 0.f)) kref = 1.f;
-            const int vexp = top ? min(max((int)top - 127, -120), 120) : 0;
-            const uint32_t hidden = __ballot_sync(0xffffffffu, blk < 0) & 255u, bad = __ballot_sync(0xffffffffu, blk >= 0 && !fine) & 255u;
-            if (w == 0 && lane == 0) {
-                TcaInfo& f = sh.info[i & 3];
-                if (is_k) { f.kref = kref; f.hidden = hidden; }
-                else { f.vexp = vexp; f.bad_v = bad; }
-                mbar_arrive(&sh.info_full[i & 3]);
+                for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const int vexp = top ? min(max((int)top - 127, -120), 120) : 0;
+                const uint32_t bad = __ballot_sync(0xffffffffu, blk >= 0 && !fine) & 255u;
+                if (lane < 8) f.vs[lane] = fine ? sc * __uint_as_float((uint32_t)(127 - vexp) << 23) : 0.f;
+                if (lane == 0) { f.vexp = vexp; f.bad_v = bad; }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.info_full[i & 3]);
             }
             if (i >= 2 && !wait(&empty[slot], (i >> 1) - 1)) break;
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const float own = __shfl_sync(0xffffffffu, sc, w + g);
-                // K over the step's largest scale; V over a power of two, a scale that is not finite as 0
-                const float r = is_k ? own / kref : fabsf(own) <= 3.402823466e38f ? own * __uint_as_float((uint32_t)(127 - vexp) << 23) : 0.f;
-                const bool plain = r == 1.f;
-                const __half2 hr = __float2half2_rn(r);
+            for (int g = 0; g < kTcaGroups; ++g) {
+                const bool plus = !(__shfl_sync(0xffffffffu, sc, w + g) < 0.f);      // a negative K scale turns its codes, so that the factor is positive
                 if (is_k) {
 #pragma unroll
                     for (int a = 0; a < 2; ++a)
@@ -318,8 +310,8 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                             uint32_t o[8];
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
-                                o[2 * k] = scaled(__byte_perm(x[k], 0x64646464u, 0x4140), plain, hr);
-                                o[2 * k + 1] = scaled(__byte_perm(x[k], 0x64646464u, 0x4342), plain, hr);
+                                o[2 * k] = turned(__byte_perm(x[k], 0x64646464u, 0x4140), plus);
+                                o[2 * k + 1] = turned(__byte_perm(x[k], 0x64646464u, 0x4342), plus);
                             }
                             uint8_t* d = sk + slot * KB + (2 * (w + g) + a) * (CG * 128) + 2 * ((lane >> 3) + 4 * j) * 128 + (lane & 7) * 16;
                             *reinterpret_cast<uint4*>(d) = make_uint4(o[0], o[1], o[2], o[3]);
@@ -335,10 +327,10 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                         for (int k = 0; k < 4; ++k) {
                             const uint32_t x = q[8 * v + 2 * k] ^ 0x80808080u, y = q[8 * v + 2 * k + 1] ^ 0x80808080u;
                             const uint32_t u0 = __byte_perm(x, y, sel0), u1 = __byte_perm(x, y, sel1);
-                            o[0][k] = scaled(__byte_perm(u0, 0x64646464u, 0x4140), plain, hr);
-                            o[1][k] = scaled(__byte_perm(u0, 0x64646464u, 0x4342), plain, hr);
-                            o[2][k] = scaled(__byte_perm(u1, 0x64646464u, 0x4140), plain, hr);
-                            o[3][k] = scaled(__byte_perm(u1, 0x64646464u, 0x4342), plain, hr);
+                            o[0][k] = unbias(__byte_perm(u0, 0x64646464u, 0x4140));
+                            o[1][k] = unbias(__byte_perm(u0, 0x64646464u, 0x4342));
+                            o[2][k] = unbias(__byte_perm(u1, 0x64646464u, 0x4140));
+                            o[3][k] = unbias(__byte_perm(u1, 0x64646464u, 0x4342));
                         }
 #pragma unroll
                         for (int d = 0; d < 4; ++d) {
@@ -354,7 +346,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
             if (i + 1 < n) load(kt0 + i + 1, blk1);
             blk = blk1; blk1 = blk2; sc = sc1;
         }
-    } else if (warp == 16) {
+    } else if (warp == kTcaMma) {
         // ------------------------------------------------ products
         if (elect_one()) {
             const uint32_t id_s = tc_idesc_f16(kTcaKeys), id_o = tc_idesc_f16(D);
@@ -402,14 +394,13 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
         for (int i = 0; i < n; ++i) {
             if (!wait(&sh.info_full[i & 3], i >> 2) || !wait(&sh.s_full[t], i)) break;
             tc_fence_after();
-            const TcaInfo info = sh.info[i & 3];
-            const float f = info.kref * scale;
+            const TcaInfo& info = sh.info[i & 3];
             const int key0 = (kt0 + i) * kTcaKeys;
             // keys of the step that the row sees: columns (a, b], less hidden groups
             const int a = z_lo - key0, b = z - key0;
             const bool edge = __any_sync(0xffffffffu, a >= 0 || b < kTcaKeys - 1) || info.hidden;
             auto seen = [&](int col) { return col <= b && col > a && !(info.hidden >> (col >> 4) & 1); };
-            // f(chunk, its sixteen scores), the next chunk on its way meanwhile
+            // f(chunk, its sixteen scores: those of a group of keys), the next chunk on its way meanwhile
             auto scores = [&](auto f) {
                 uint32_t r[2][16];
                 tc_ld16_nowait(s_at, r[0]);
@@ -420,17 +411,30 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                     f(c, r[c & 1]);
                 }
             };
-            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};           // four chains
-            if (edge) scores([&](int c, const uint32_t (&r)[16]) {
+            float tops[8];                                      // of the groups
+            auto highest = [&](auto masked) {
+                scores([&](int c, const uint32_t (&r)[16]) {
+                    float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};         // four chains
 #pragma unroll
-                for (int k = 0; k < 16; ++k) tops[k & 3] = seen(16 * c + k) ? fmaxf(tops[k & 3], __uint_as_float(r[k])) : tops[k & 3];
-            });
-            else scores([&](int, const uint32_t (&r)[16]) {
+                    for (int k = 0; k < 16; k += 2) {
+                        float x = __uint_as_float(r[k]), y = __uint_as_float(r[k + 1]);
+                        if constexpr (decltype(masked)::value) {
+                            x = seen(16 * c + k) ? x : -INFINITY;
+                            y = seen(16 * c + k + 1) ? y : -INFINITY;
+                        }
+                        t4[k >> 1 & 3] = fmaxf(t4[k >> 1 & 3], fmaxf(x, y));
+                    }
+                    tops[c] = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                });
+            };
+            if (edge) highest(std::true_type());
+            else highest(std::false_type());
+            float fk[8], top = -INFINITY;                       // the factors are read once: between the TMEM loads they would be waited for
 #pragma unroll
-                for (int k = 0; k < 16; k += 2) tops[k >> 1 & 3] = fmaxf(tops[k >> 1 & 3], fmaxf(__uint_as_float(r[k]), __uint_as_float(r[k + 1])));
-            });
-            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-            top = top == -INFINITY ? top : top * f;
+            for (int c = 0; c < 8; ++c) {
+                fk[c] = info.ks[c] * scale;
+                top = tops[c] != -INFINITY ? fmaxf(top, tops[c] * fk[c]) : top;         // -inf may meet a factor of 0
+            }
             const bool grows = top > m + kAttnSlack, scale_grows = info.vexp > vrun + kTcaScaleSlack;
             if (__any_sync(0xffffffffu, grows) || scale_grows) {
                 const float m_new = fmaxf(m, top);
@@ -458,8 +462,12 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
             }
             const float m_safe = m == -INFINITY ? 0.f : m, shift = kTcaLift + (float)max(info.vexp - vrun, -100) - m_safe;
             f2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};
+            float fv[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) fv[c] = info.vs[c];
             auto weights = [&](auto masked) {
                 scores([&](int c, const uint32_t (&r)[16]) {
+                    const float f = fk[c], v = fv[c];
                     uint32_t u[8];
 #pragma unroll
                     for (int k = 0; k < 16; k += 2) {
@@ -470,7 +478,8 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                             e1 = seen(16 * c + k + 1) ? e1 : 0.f;
                         }
                         sums[k >> 1 & 1] = fadd2(sums[k >> 1 & 1], f2{e0, e1});
-                        u[k >> 1] = pack_half2(e0, e1);
+                        const f2 w = ffma2(f2{e0, e1}, f2{v, v}, f2{0.f, 0.f});
+                        u[k >> 1] = pack_half2(w.x, w.y);
                     }
                     tc_st8(s_at + 8 * c, u);                    // over scores that were read
                 });
@@ -520,7 +529,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 16) {
+    if (warp == kTcaMma) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }

@@ -53,7 +53,7 @@ struct AppendParams {
     int blocks, kv_heads, shift, dim, tokens, q_heads;
     int q_groups, q_group;     // groups of query heads, heads in one
     int q_ctas, kv_tile;       // CTAs of the queries' part, which come last
-    int x_f32, y_f32, vec;     // vec: pointers and strides allow 16-byte accesses
+    int vec;                   // pointers and strides allow 16-byte accesses
     RopeParams rope;
 };
 

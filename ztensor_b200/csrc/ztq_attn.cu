@@ -117,7 +117,7 @@ size_t ztq_attn_q8_workspace_bytes(int tokens, int sequences, int max_new, int q
 cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_head, long long y_token, long long y_head, int tokens, int q_heads,
                         const int* query_start, const int* kv_len, const int* block_table, int sequences, int table_width, int max_new, int window,
                         unsigned scale_bits, const ZtqKvCache* cache, void* workspace, size_t workspace_bytes, int flags, cudaStream_t stream) {
-    if (!q || !y || !query_start || !kv_len || !block_table || !cache || !cache->k || !cache->v || !cache->k_scale || !cache->v_scale || !workspace) return cudaErrorInvalidValue;
+    if ((tokens != 0 && (!q || !y)) || !query_start || !kv_len || !block_table || !cache || !cache->k || !cache->v || !cache->k_scale || !cache->v_scale || !workspace) return cudaErrorInvalidValue;
     const int shift = attn_block_shift(cache->block_size), dim = cache->head_dim;
     if (shift < 0 || (dim != 64 && dim != 128 && dim != 256) || cache->blocks <= 0 || cache->kv_heads <= 0) return cudaErrorInvalidValue;
     if (cache->block_stride < (long long)cache->kv_heads * cache->block_size * dim || cache->block_stride % 16) return cudaErrorInvalidValue;

@@ -34,10 +34,10 @@ static bool cache_ok(const ZtqKvCache* c) {
 }
 
 // Rotary arguments -> parameters; false where they do not fit heads of `dim`.
-static bool rope_params(const void* table, int table_rows, int rot_dim, const int* positions, int dim, int flags, RopeParams& r) {
+static bool rope_params(const void* table, int table_rows, int rot_dim, const int* positions, int tokens, int dim, int flags, RopeParams& r) {
     r = RopeParams{};
     if (!table) return true;
-    if (!aligned16(table) || table_rows <= 0 || rot_dim < 16 || rot_dim % 16 || rot_dim > dim || !positions) return false;
+    if (!aligned16(table) || table_rows <= 0 || rot_dim < 16 || rot_dim % 16 || rot_dim > dim || (tokens != 0 && !positions)) return false;
     r.table = static_cast<const float2*>(table);
     r.positions = positions;
     r.table_rows = table_rows;
@@ -130,12 +130,12 @@ cudaError_t ztq_rope_table(void* table, int first, int rows, const ZtqRopeSpec* 
 
 cudaError_t ztq_rope(const void* x, void* y, int tokens, int heads, int head_dim, long long x_token, long long x_head, long long y_token,
                      long long y_head, const void* table, int table_rows, int rot_dim, const int* positions, int flags, cudaStream_t stream) {
-    if (!x || !y || tokens < 0 || heads <= 0 || head_dim < 16 || head_dim > 256 || head_dim % 16 || !table) return cudaErrorInvalidValue;
+    if ((tokens != 0 && (!x || !y)) || tokens < 0 || heads <= 0 || head_dim < 16 || head_dim > 256 || head_dim % 16 || !table) return cudaErrorInvalidValue;
     if (flags & ~(ZTQ_X_F32 | ZTQ_Y_F32 | ZTQ_NO_PDL | ZTQ_ROPE_PAIRS)) return cudaErrorInvalidValue;
     RopeParams r;
-    if (!rope_params(table, table_rows, rot_dim, positions, head_dim, flags, r)) return cudaErrorInvalidValue;
+    if (!rope_params(table, table_rows, rot_dim, positions, tokens, head_dim, flags, r)) return cudaErrorInvalidValue;
     const bool xf = flags & ZTQ_X_F32, yf = flags & ZTQ_Y_F32;
-    if (x == y && (xf != yf || x_token != y_token || x_head != y_head)) return cudaErrorInvalidValue;
+    if (x && x == y && (xf != yf || x_token != y_token || x_head != y_head)) return cudaErrorInvalidValue;
     const DeviceInfo dev = device_info();
     if (dev.major < 10) return cudaErrorNoKernelImageForDevice;
     if (tokens == 0) return cudaSuccess;
@@ -152,12 +152,12 @@ cudaError_t ztq_rope_append_q8(const void* q, const void* k, const void* v, void
                                long long k_head, long long v_token, long long v_head, long long qo_token, long long qo_head, int tokens, int q_heads,
                                const void* table, int table_rows, int rot_dim, const int* positions, const int* slots, const ZtqKvCache* cache,
                                int flags, cudaStream_t stream) {
-    if (!k || !v || !slots || tokens < 0 || q_heads < 0 || (q_heads > 0 && (!q || !q_out)) || !cache_ok(cache)) return cudaErrorInvalidValue;
+    if ((tokens != 0 && (!k || !v || !slots || (q_heads > 0 && (!q || !q_out)))) || tokens < 0 || q_heads < 0 || !cache_ok(cache)) return cudaErrorInvalidValue;
     if (flags & ~(ZTQ_X_F32 | ZTQ_Y_F32 | ZTQ_NO_PDL | ZTQ_ROPE_PAIRS)) return cudaErrorInvalidValue;
     AppendParams p = {};
-    if (!rope_params(table, table_rows, rot_dim, positions, cache->head_dim, flags, p.rope)) return cudaErrorInvalidValue;
+    if (!rope_params(table, table_rows, rot_dim, positions, tokens, cache->head_dim, flags, p.rope)) return cudaErrorInvalidValue;
     const bool xf = flags & ZTQ_X_F32, yf = flags & ZTQ_Y_F32;
-    if (q_heads > 0 && q == q_out && (xf != yf || q_token != qo_token || q_head != qo_head)) return cudaErrorInvalidValue;
+    if (q_heads > 0 && q && q == q_out && (xf != yf || q_token != qo_token || q_head != qo_head)) return cudaErrorInvalidValue;
     const DeviceInfo dev = device_info();
     if (dev.major < 10) return cudaErrorNoKernelImageForDevice;
     if (tokens == 0) return cudaSuccess;
@@ -177,8 +177,6 @@ cudaError_t ztq_rope_append_q8(const void* q, const void* k, const void* v, void
     p.dim = cache->head_dim;
     p.tokens = tokens;
     p.q_heads = q_heads;
-    p.x_f32 = xf;
-    p.y_f32 = yf;
     p.vec = wide(p.k, xf) && wide(p.v, xf) && (q_heads == 0 || (wide(p.q, xf) && wide(p.qo, yf)));
     const int tiles = ceil_div(tokens, kTokenTile);
     p.q_group = q_heads ? head_group(q_heads, tiles, p.dim, dev.sms) : 1;
@@ -194,7 +192,7 @@ cudaError_t ztq_rope_append_q8(const void* q, const void* k, const void* v, void
 }
 
 cudaError_t ztq_kv_read_q8(const ZtqKvCache* cache, const int* slots, int tokens, void* k_out, void* v_out, int flags, cudaStream_t stream) {
-    if (!cache_ok(cache) || !slots || tokens < 0 || (!k_out && !v_out) || !aligned16(k_out) || !aligned16(v_out)) return cudaErrorInvalidValue;
+    if (!cache_ok(cache) || (tokens != 0 && (!slots || (!k_out && !v_out))) || tokens < 0 || !aligned16(k_out) || !aligned16(v_out)) return cudaErrorInvalidValue;
     if (flags & ~(ZTQ_Y_F32 | ZTQ_NO_PDL)) return cudaErrorInvalidValue;
     const DeviceInfo dev = device_info();
     if (dev.major < 10) return cudaErrorNoKernelImageForDevice;
@@ -220,7 +218,7 @@ cudaError_t ztq_kv_read_q8(const ZtqKvCache* cache, const int* slots, int tokens
 
 cudaError_t ztq_sample(const void* logits, long long row_stride, int rows, int vocab, const float* temperature, const int* top_k,
                        const float* top_p, const float* min_p, const float* uniform, int* token, float* logprob, int flags, cudaStream_t stream) {
-    if (!logits || !uniform || !token || rows < 0 || vocab <= 0 || vocab > ZTQ_SAMPLE_MAX_VOCAB || (rows > 1 && row_stride < vocab)) return cudaErrorInvalidValue;
+    if ((rows != 0 && (!logits || !uniform || !token)) || rows < 0 || vocab <= 0 || vocab > ZTQ_SAMPLE_MAX_VOCAB || (rows > 1 && row_stride < vocab)) return cudaErrorInvalidValue;
     if (rows > 0x7fffffff / kSampleMaxCluster) return cudaErrorInvalidValue;
     if (flags & ~(ZTQ_X_F32 | ZTQ_NO_PDL)) return cudaErrorInvalidValue;
     const DeviceInfo dev = device_info();
