@@ -644,6 +644,45 @@ def test_decode_steps_together(captured):
     no_error()
 
 
+def test_projection_stack_with_attention():
+    """Decode steps of an 8B-shaped layer, captured once: O reads the attention over what the QKV projection wrote in every
+    step; a sequence that ends gives its blocks back and begins anew."""
+    from ztensor_b200.stack import DecodeAttention, ProjectionStack
+    st = ProjectionStack("llama3-8b", batch=2, layers=1)
+    att = DecodeAttention(st, blocks=5, block_size=16, max_positions=64)
+    st.step(attention=att)                       # loads the kernels
+    att.ctx.zero_(), att.ring_state.copy_(torch.tensor([0, 5], device=DEV))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        st.step(attention=att)
+    torch.cuda.synchronize()
+    att.ctx.zero_(), att.ring_state.copy_(torch.tensor([0, 5], device=DEV))
+    rng, held, table = U.seeded(15), [[], []], host(att.rope)
+    for step in range(40):
+        att.new.copy_(torch.tensor([1, -1 if step == 20 else 1], device=DEV))
+        st.x["qkv"].copy_(dev(rng.standard_normal((2, 4096))))
+        before = st.x["o"].clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert att.status.tolist() == [0, 0] and att.positions.tolist()[0] == len(held[0])
+        if step == 20:
+            held[1] = []
+            assert torch.equal(st.x["o"][1], before[1])
+        # the queries were rotated in place; keys and values stand in y as the projection left them
+        y, out = host(st.y["qkv"]).reshape(2, 48, 128), host(st.x["o"]).reshape(2, 32, 128)
+        for b in range(1 if step == 20 else 2):
+            held[b].append((R.rope(y[b:b + 1, 32:40], table, np.array([len(held[b])]), False)[0], y[b, 40:]))
+            k, v = (np.stack([r[j] for r in held[b]]) for j in (0, 1))
+            for h in range(0, 32, 5):
+                kk, vv = k[:, h // 4], v[:, h // 4]
+                ref, mean, _, _ = R.attention(y[b:b + 1, h], kk, vv, len(kk) - 1, 128 ** -0.5, 0)
+                key_step, val_step = 2 * np.abs(kk).max() / 127, 2 * np.abs(vv).max() / 127       # as in the loop of decode steps above
+                tol = (np.exp(2 * 128 ** -0.5 * key_step * np.abs(y[b, h]).sum()) - 1) * 2 * mean + val_step + 4 * HALF16 * mean
+                assert (np.abs(out[b, h] - ref[0]) <= tol[0]).all()
+    no_error()
+
+
 def test_calls_without_rows_do_nothing():
     cache = random_cache(U.seeded(14), 4, 2, 16, 64)
     before = [t.clone() for t in cache.tensors]

@@ -13,7 +13,9 @@ Weights are GPTQ-style 4-bit, group 128 along K (tensor/quantized_gptq.go layout
 residency layout of include/ztq.h), quantized on the device by the library's own
 quantizer from seeded N(0, 0.02) float32 matrices.  Only the projections run:
 activations between them are fixed fp16 N(0,1) buffers, as the benchmark
-configuration specifies.  The all-reduce after O and down is NCCL (through
+configuration specifies, unless a step is given a DecodeAttention: then the QKV
+projection's output is rotated, appended to the layer's paged 8-bit cache and
+attended over, and the result is what O reads.  The all-reduce after O and down is NCCL (through
 torch.distributed) on the same stream as the kernels, so the whole step can be
 recorded into one CUDA graph per rank.
 """
@@ -82,6 +84,40 @@ def quantize_matrix(n: int, k: int, seed: int, device, awq: bool = False, chunk_
     if with_packed:
         return qdata, meta, packed, moff
     return qdata, meta
+
+
+class DecodeAttention:
+    """What a decode loop keeps between steps for the attention of a ProjectionStack: the sequences' lengths and block
+    tables, the pool of free blocks, one paged 8-bit cache per layer, the rotary table and the workspace.  Every step each
+    of the stack's `batch` sequences brings one token; set `new` to -1 to end a sequence (its blocks go back to the pool,
+    its rows of that step are padding) and to 0 to let it wait."""
+
+    def __init__(self, stack: "ProjectionStack", blocks: int, block_size: int = 64, max_positions: int = 8192, rope_base: float = 500000.0, **rope_scaling):
+        _, _, _, qh, kvh = SHAPES[stack.model]
+        self.q_heads, self.kv_heads, self.dim, self.block_size = qh // stack.world, kvh // stack.world, 128, block_size
+        b, dev = stack.batch, stack.device
+        i32 = lambda *n: torch.zeros(*n, dtype=torch.int32, device=dev)  # noqa: E731
+        self.ctx, self.new, self.table = i32(b), i32(b) + 1, i32(b, -(-max_positions // block_size)) - 1
+        self.ring, self.ring_state = torch.arange(blocks, dtype=torch.int32, device=dev), i32(2)
+        self.ring_state[1] = blocks
+        self.kv_len, self.start, self.positions, self.slots, self.status = i32(b), i32(b + 1), i32(b), i32(b), i32(b)
+        self.caches = [K.KvCache.empty(blocks, self.kv_heads, block_size, self.dim, device=dev) for _ in stack.layers]
+        self.rope = K.rope_table(max_positions, self.dim, rope_base, **rope_scaling)
+        self.workspace = torch.empty(K.attn_q8_workspace_bytes(b, b, 1, self.q_heads, self.kv_heads, self.dim), dtype=torch.uint8, device=dev)
+
+    def begin_step(self):
+        """Blocks, slots, positions and lengths of the step (lengths advance)."""
+        K.kv_plan(self.ctx, self.new, self.table, self.ring, self.ring_state, self.ring_state, self.ctx, self.kv_len, self.start, self.positions, self.slots, self.status,
+                  self.block_size)
+
+    def run(self, layer: int, qkv, out):
+        """qkv [batch, (q_heads + 2 kv_heads) * 128], rows in the order of the sequences that bring a token, -> out [batch, q_heads * 128]."""
+        heads = qkv.view(qkv.shape[0], self.q_heads + 2 * self.kv_heads, self.dim)
+        q, k, v = heads.split([self.q_heads, self.kv_heads, self.kv_heads], 1)
+        cache = self.caches[layer]
+        K.rope_append_q8(q, k, v, q, self.slots, cache, self.rope, self.positions)
+        K.attn_q8(q, out.view(out.shape[0], self.q_heads, self.dim), self.start, self.kv_len, self.table, cache, self.workspace, 1, self.dim ** -0.5)
+        return out
 
 
 class ProjectionStack:
@@ -167,12 +203,17 @@ class ProjectionStack:
             self._nccl_all_reduce(y)
         return y
 
-    def step(self, fused=None):
+    def step(self, fused=None, attention: DecodeAttention | None = None):
         """One token-step: every projection of every layer, in order, on the current stream.
 
         fused: a collective.FusedAllReduce -> the all-reduce after O and down runs inside the
-        GEMV kernel; None -> NCCL all-reduce (torch.distributed) after the kernel."""
-        for layer in self.layers:
+        GEMV kernel; None -> NCCL all-reduce (torch.distributed) after the kernel.
+        attention: its rotary positions, cache append and attention run between QKV and O of every layer."""
+        if attention is not None:
+            attention.begin_step()
+        for li, layer in enumerate(self.layers):
             for p in layer:
                 self.run_projection(p, fused)
+                if attention is not None and p.name == "qkv":
+                    attention.run(li, self.y["qkv"], self.x["o"])
         return self.y["down"]
