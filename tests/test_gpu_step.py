@@ -340,7 +340,10 @@ def test_attn_windows_types_and_strides(f32, layout, window, lens):
     attn_run(lens, 2, 5, 32, 64 if window % 2 else 128, f32=f32, window=window, layout=layout, seed=window)
 
 
-@pytest.mark.parametrize("lens,heads,group,dim", [([(20001, 1)], 8, 8, 128), ([(9000, 1), (3, 1), (5000, 1)], 1, 1, 64), ([(5000, 3)], 2, 4, 256), ([(3000, 260)], 2, 4, 128),
+MIXED = [(300 + 7 * i, 1 if i % 3 else 30 + i) for i in range(40)]         # more heads than SMs: both kernels share the batch
+
+
+@pytest.mark.parametrize("lens,heads,group,dim", [(MIXED, 4, 4, 64), (MIXED, 4, 3, 128), ([(20001, 1)], 8, 8, 128), ([(9000, 1), (3, 1), (5000, 1)], 1, 1, 64), ([(5000, 3)], 2, 4, 256), ([(3000, 260)], 2, 4, 128),
                                                   ([(700, 1)] * 90, 2, 8, 64)])
 def test_attn_long(lens, heads, group, dim):
     attn_run(lens, heads, group, 64, dim, seed=len(lens))

@@ -53,19 +53,23 @@ static cudaError_t launch_dim(const AttnParams& p, int nt, bool split, int sms, 
 }
 
 // Prompts: sequences with more than kTcMinRows rows per kv head go to the tensor-core kernel (fp16, heads of 64 and 128).
+// With few sequences all of them do: a launch of its own for those with few rows would cost more than their 256-row items
+// (three sequences of 91, 26 and 91 tokens: 58 us with both kernels and their joins, 33 with one).
 constexpr int kTcMinRows = 64;
 
 struct TcPlan {
     long long items = 0;          // CTAs of one split; 0: the kernel is not used
     int splits = 1;
+    bool all = false;             // takes every sequence
     size_t bytes = 0;             // of its workspace
 };
 static TcPlan tc_plan(int tokens, int sequences, long long most_rows, int group, int kv_heads, int head_dim, int sms) {
     TcPlan t;
     if (most_rows <= kTcMinRows || head_dim > 128) return t;
-    // an item is 256 rows of a sequence: full ones, and one begun by each sequence that has enough rows
+    t.all = sequences == 1 || (long long)sequences * kv_heads <= sms;
+    // an item is 256 rows of a sequence: full ones, and one begun by each sequence that is taken
     const long long rows = (long long)tokens * group, full = rows / kTcaRows;
-    const long long begun = sequences == 1 ? 1 : std::min<long long>(sequences, rows / (kTcMinRows + 1) + 1);
+    const long long begun = t.all ? sequences : std::min<long long>(sequences, rows / (kTcMinRows + 1) + 1);
     t.items = (full + begun) * kv_heads;
     // few items: cut their keys so that every SM has a CTA
     const long long few = (full > 0 ? full : 1) * kv_heads;
@@ -78,8 +82,8 @@ template <int D>
 static cudaError_t launch_tc(const AttnParams& p, const TcPlan& plan, cudaStream_t stream, bool pdl) {
     TcaParams tp;
     tp.a = p;
-    // a split is worth four steps
-    tp.splits = (int)std::max<long long>(1, std::min<long long>(plan.splits, (((long long)p.width << p.shift) + 4 * kTcaKeys - 1) / (4 * kTcaKeys)));
+    // a split is worth eight steps: the join takes as long as two
+    tp.splits = (int)std::max<long long>(1, std::min<long long>(plan.splits, ((long long)p.width << p.shift) / (8 * kTcaKeys)));
     tp.parts = p.parts;
     static std::atomic<unsigned> done{0};
     auto kern = attn_tc_kernel<D>;
@@ -169,10 +173,9 @@ cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_h
         const TcPlan plan = tc_plan(tokens, sequences, (long long)max_new * p.group, p.group, p.kv_heads, dim, dev.sms);
         if (plan.items > 0x7fffffff) return cudaErrorInvalidValue;
         if (plan.items > 0) {
-            // a single sequence goes there whatever it turns out to bring; several are told apart on the device
-            if (sequences > 1) p.min_rows = kTcMinRows + 1;
+            if (!plan.all) p.min_rows = kTcMinRows + 1;          // told apart on the device, where the lengths are
             cudaError_t e = dim == 64 ? launch_tc<64>(p, plan, stream, pdl) : launch_tc<128>(p, plan, stream, pdl);
-            if (e != cudaSuccess || sequences == 1) return e;
+            if (e != cudaSuccess || plan.all) return e;
             p.min_rows = 1;
             p.max_rows = kTcMinRows;
         }
