@@ -217,6 +217,20 @@ def test_append(x32, tokens, heads, qh, size, dim, rot, layout):
     no_error()
 
 
+@pytest.mark.parametrize("x32", [False, True])
+def test_append_rotates_queries_into_the_other_type(x32):
+    rng = U.seeded(16)
+    cache, table = random_cache(rng, 40, 2, 16, 64), K.rope_table(100, 64, 10000.0)
+    x = dev(rng.standard_normal((21, 8, 64)), torch.float32 if x32 else torch.float16)
+    q, k, v = x.split([4, 2, 2], 1)
+    out = torch.zeros(21, 4, 64, dtype=torch.float16 if x32 else torch.float32, device=DEV)
+    pos = rng.integers(0, 100, 21).astype(np.int32)
+    K.rope_append_q8(q, k, v, out, dev(np.arange(21, dtype=np.int32) * 16), cache, table, dev(pos))
+    ref = R.rope(host(q), host(table), pos, False)
+    assert (np.abs(host(out) - ref) <= 3 * HALF32 * 2 * np.abs(host(q)).max() + (HALF16 * np.abs(ref) + 2.0 ** -25 if x32 else 0)).all()
+    no_error()
+
+
 def test_append_grows_a_block_step_by_step():
     """One token per step into one block, each larger than all before: every step rounds the old rows once."""
     cache = K.KvCache.empty(2, 1, 16, 64)
@@ -293,15 +307,16 @@ def attn_check(lens, cache, table, start, q, y, scale, window, f32):
             kk = (k[blocks, h] * ks[blocks, h][:, None, None]).reshape(-1, cache.head_dim)[:n]
             vv = (v[blocks, h] * vs[blocks, h][:, None, None]).reshape(-1, cache.head_dim)[:n]
             for g in range(h * group, (h + 1) * group):
-                ref, mean, size, sums = R.attention(qh[row:row + a, g], kk, vv, n - a, scale, window)
+                ref, mean, size, _ = R.attention(qh[row:row + a, g], kk, vv, n - a, scale, window)
                 # scores: fp32 sums of exact products (q in one or two fp16 terms), D / 16 + 2 roundings of the running
                 # sum; weights: the half step of fp16, or of two terms; sums and division in fp32; the output's half step.
-                # A weight far below the largest ends at fp16's last step: it is held times 2^7, the last half step is 2^-25,
-                # so a weight of the largest's 2^-21 or less is off by up to 2^-32 of the largest, whose weight is at least 1
-                # of the sum's parts: 2^-32 sum |v| in all
+                # A weight far below the largest ends at fp16's last step: weights times the V scale over a power of two, at
+                # most the largest scale of the cache, are held times 2^4 (fp32: 2^12) and the last half step is 2^-25, so
+                # each is off by up to 2^-29 (2^-37) of the largest, whose weight is at least 1 of the sum's parts
+                ends = (2.0 ** -37 if f32 else 2.0 ** -29) * np.abs(vs).max() * np.abs(v[blocks, h]).reshape(-1, cache.head_dim)[:n].sum(0)
                 term = 2.0 ** -22 if f32 else 0.0
                 weight = (cache.head_dim / 16 + 2) * 2 * HALF32 * size + term * size + (4 * 2.0 ** -22 if f32 else HALF16) + 64 * HALF32
-                tol = 2 * weight * mean + 2.0 ** -32 * sums + (0 if f32 else HALF16 * np.abs(ref) + 2.0 ** -25) + 2.0 ** -40
+                tol = 2 * weight * mean + ends + (0 if f32 else HALF16 * np.abs(ref) + 2.0 ** -25) + 2.0 ** -40
                 assert (np.abs(got[row:row + a, g] - ref) <= tol).all(), (b, g, float(np.max(np.abs(got[row:row + a, g] - ref) / tol)))
         row += a
     assert (got[row:] == 0.5).all()              # rows behind the last sequence
@@ -338,6 +353,21 @@ def test_attn(dim, group, heads, lens):
 @pytest.mark.parametrize("lens", [ONE, FEW, MANY], ids=["one", "few", "many"])
 def test_attn_windows_types_and_strides(f32, layout, window, lens):
     attn_run(lens, 2, 5, 32, 64 if window % 2 else 128, f32=f32, window=window, layout=layout, seed=window)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("x32,y32", [(True, True), (True, False), (False, True)])
+@pytest.mark.parametrize("lens", [ONE[2:6], FEW, MANY], ids=["one", "few", "many"])
+def test_attn_types_apart(dim, x32, y32, lens):
+    """Queries and outputs of different types; windows as large as an int holds."""
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(dim), lens, 2, 3, 16, dim, torch.float32 if x32 else torch.float16)
+    y = torch.full(q.shape, 0.5, dtype=torch.float32 if y32 else torch.float16, device=DEV)
+    most = max(a for _, a in lens)
+    ws = torch.empty(K.attn_q8_workspace_bytes(q.shape[0], len(lens), most, 6, 2, dim), dtype=torch.uint8, device=DEV)
+    for window in (0, 2 ** 31 - 1, 17):
+        K.attn_q8(q, y, start, kv_len, table, cache, ws, most, 0.1, window)
+        attn_check(lens, cache, table, start, q, y, 0.1, min(window, 1 << 20), y32)
+    no_error()
 
 
 MIXED = [(300 + 7 * i, 1 if i % 3 else 30 + i) for i in range(40)]         # more heads than SMs: both kernels share the batch

@@ -10,7 +10,8 @@
 //   One CTA per SM: a producer warp keeps a ring of steps of 128 tokens (32 KB at D = 128) filled by tiled TMA copies, one
 // per block, and looks up block table and scales one step ahead; the other warps take 16 tokens of a step in turn.  Twelve of
 // them where 128 registers suffice: a warp's tile is a chain of 380 instructions that eight warps leave half hidden
-// (64 sequences of 3000 to 12000 tokens, 958 MB: 211 us with eight).
+// (64 sequences of 3000 to 12000 tokens, 958 MB: 211 us with eight,
+// 192 with twelve and the look-ahead of the producer).
 //   S^T = K Q^T and Y^T = V^T P^T by mma.sync m16n8k16 with the TOKENS (then the dims) as M and the rows as N = 8: a
 // decode step has 4 to 8 rows per kv head, which as M would waste half of every instruction and more.
 //   The contraction index may be permuted as long as both operands agree, so every lane reads 16 contiguous bytes of the
@@ -19,9 +20,9 @@
 // pairs two tokens' codes by byte permutes.  P^T is the transposed accumulator of S^T (movmatrix).  tau = 0 5 2 7 4 1 6 3:
 // with the copies' 128-byte swizzle both reads are free of bank conflicts (even and odd g differ in bit 2 of the row, even
 // rows of the c's are all different).  A code becomes fp16 exactly: 0x6400 | (code + 128) is 1152 + code.
-//   Online softmax per warp: the running maximum m moves only when some score exceeds it by more than kSlack in the
-// exponent (one vote per 16 tokens instead of a reduction); p = 2^(s - m + kLift) stays below 2^15, inside fp16, and a
-// weight of 2^-19 of the largest is still a normal number.  Scores, maxima, sums and accumulators are fp32; p is rounded to
+//   Online softmax per warp: the running maximum m moves only when some score exceeds it by more than a slack of 8 in the
+// exponent (one vote per 16 tokens instead of a reduction); p = 2^(s - m + 4) then stays inside fp16 and ends at 2^-28 of the
+// largest weight.  Scores, maxima, sums and accumulators are fp32; p is rounded to
 // fp16 for the second product (relative 2^-11, against fp16 outputs with the same step).  With fp32 inputs or outputs
 // (SPLIT) q and p go in as two fp16 terms each, 22 bits.
 //   A tile of 16 tokens lies in one block (block sizes are multiples of 16), so its scales are two scalars: sk goes into
@@ -41,9 +42,13 @@ constexpr int kAttnMaxSeqs = 4096;
 constexpr int kAttnStep = 128;                      // tokens of a step: eight tiles of 16, dealt to the warps in turn
 constexpr int kAttnMinSteps = 1;                    // steps a CTA gets at least
 constexpr uint32_t kAttnHidden = 0xfffe5afeu;       // in place of a K scale: 16 tokens without a block (a NaN no arithmetic makes)
-constexpr float kAttnSlack = 8.f;                   // how far a score may exceed the running maximum before that moves
-constexpr float kAttnLift = 5.f;
-constexpr int kAttnScaleSlack = 2;                  // how far a block's V scale may exceed the running power of two: p < 2^(8 + 5 + 2)
+// A score may exceed the running maximum by `slack` before that moves, a block's V scale the running power of two by
+// kAttnScaleSlack, and a scale is below twice its power of two: p = 2^(s - m + lift) sv / 2^vrun < 2^(slack + lift + 3), which
+// has to stay below 2^16.  With two terms per weight (SPLIT) every bit that the slack does not take goes to small weights.
+__host__ __device__ constexpr float attn_slack(bool split) { return split ? 0.f : 8.f; }
+__host__ __device__ constexpr float attn_lift(bool split) { return split ? 12.f : 4.f; }
+constexpr int kAttnScaleSlack = 2;
+static_assert(attn_slack(false) + attn_lift(false) + kAttnScaleSlack + 1 < 16 && attn_slack(true) + attn_lift(true) + kAttnScaleSlack + 1 < 16, "p stays below 2^15");
 
 struct AttnParams {
     const void* q;
@@ -88,7 +93,7 @@ __device__ __forceinline__ void attn_span(const AttnParams& p, const AttnSeq& s,
     const int base = s.len - s.fresh;               // position of the first new token
     const int a = base + r0 / p.group, z = base + (r1 - 1) / p.group;
     hi = min(max(z + 1, 0), s.len);
-    lo = p.window > 0 ? min(max(a - p.window + 1, 0), hi) : 0;
+    lo = p.window > 0 ? (int)min(max((long long)a - p.window + 1, 0ll), (long long)hi) : 0;
 }
 __device__ __forceinline__ int attn_steps(int lo, int hi, int step) {
     return max(1, (hi + step - 1) / step - lo / step);          // an item without keys still writes its zeros
@@ -290,7 +295,7 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
     if (warp == kAttnWarps) {
         // ------------------------------------------------ producer: lane 8 k + j looks after tokens 16 j .. of the k-th of four
         // steps; their blocks and scales are fetched while the four before are issued (two loads that wait for one another
-        // would otherwise take as long as a step's copies: 211 -> 170 us on the case above)
+        // would otherwise take as long as a step's copies)
         const int per = 1 << (p.shift - 4);                     // 16-token groups of a block: the first of them in a step copies
         int n = 0;                                              // steps issued
         for (long long w = w0; w < w_end;) {
@@ -473,7 +478,7 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
                         const bool seen = !hidden && key <= z && (p.window <= 0 || key > z - p.window);
                         sc[t][i] = seen ? sc[t][i] : -INFINITY;
                     }
-                    grows |= sc[t][i] > m[t][i & 1] + kAttnSlack;
+                    grows |= sc[t][i] > m[t][i & 1] + attn_slack(SPLIT);
                 }
             if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
@@ -521,7 +526,7 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
             uint32_t ph[NT][2], pl[SPLIT ? NT : 1][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const float shift0 = kAttnLift - (m[t][0] == -INFINITY ? 0.f : m[t][0]), shift1 = kAttnLift - (m[t][1] == -INFINITY ? 0.f : m[t][1]);
+                const float shift0 = attn_lift(SPLIT) - (m[t][0] == -INFINITY ? 0.f : m[t][0]), shift1 = attn_lift(SPLIT) - (m[t][1] == -INFINITY ? 0.f : m[t][1]);
                 float e[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {

@@ -11,7 +11,7 @@
 //
 // Roles of the warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread is a row: TMEM lane), then kTcaConv for K codes ->
 // operand and kTcaConv for V (loaded one step ahead, their blocks and scales two), the last issues the products.  The two tiles alternate: while one is in its softmax
-// the tensor cores work for the other.  The running maximum moves only when a score exceeds it by more than kAttnSlack
+// the tensor cores work for the other.  The running maximum moves only when a score exceeds it by more than kTcaSlack
 // (then the row's O is rescaled in TMEM), as does the reference of the V scales.
 // Operands stand in the canonical K-major layout without swizzle: core matrices of 8 rows x 16 bytes, 128 bytes apart along
 // the contraction; both store patterns below are free of bank conflicts.
@@ -35,8 +35,9 @@ constexpr int kTcaConv = 4;                      // warps that convert K, and as
 constexpr int kTcaGroups = 8 / kTcaConv;         // groups of 16 keys that each of them takes
 constexpr int kTcaMma = 8 + 2 * kTcaConv;
 constexpr int kTcaThreads = 32 * (kTcaMma + 1);
-constexpr float kTcaLift = 4.f;                 // with kAttnSlack, kTcaScaleSlack and the scales' significands below 2: P < 2^15
+constexpr float kTcaLift = 4.f, kTcaSlack = 8.f;  // with kTcaScaleSlack and the scales' significands below 2: P < 2^15
 constexpr int kTcaScaleSlack = 2;
+static_assert(kTcaLift + kTcaSlack + kTcaScaleSlack + 1 < 16, "P stays below 2^15");
 
 struct __align__(16) TcaInfo {                  // one step's factors, by groups of 16 keys
     float ks[8], vs[8];                         // |K scale|; V scale / 2^vexp, 0 where it is not finite
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                 fk[c] = info.ks[c] * scale;
                 top = tops[c] != -INFINITY ? fmaxf(top, tops[c] * fk[c]) : top;         // -inf may meet a factor of 0
             }
-            const bool grows = top > m + kAttnSlack, scale_grows = info.vexp > vrun + kTcaScaleSlack;
+            const bool grows = top > m + kTcaSlack, scale_grows = info.vexp > vrun + kTcaScaleSlack;
             if (__any_sync(0xffffffffu, grows) || scale_grows) {
                 const float m_new = fmaxf(m, top);
                 float fix = m == -INFINITY ? 0.f : ex2(m - m_new);
