@@ -276,6 +276,10 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
     __shared__ int failed;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
 
+    if (tid == 32 * kAttnWarps) {                               // the maps are on their way while the lengths are read
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&k_map)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)) : "memory");
+    }
     if (tid == 0) {
         for (int i = 0; i < Ring::kStages; ++i) {
             mbar_init(&full[i], 1);

@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanParams 
     const int released = (int)min(given_before, (long long)(p.pool - count));
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 
+    auto wrap = [&](int i) { return i >= p.pool ? i - p.pool : i; };
     // per sequence: lengths and status
     const int stride = ranks * blockDim.x, at = rank * blockDim.x + tid;
     for (int b = at; b < p.seqs; b += stride) {
@@ -141,11 +142,21 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanParams 
     for (int b = rank * (blockDim.x >> 5) + (tid >> 5); b < p.seqs; b += warps) {
         const PlanSeq q = seq[b];
         int* row = p.block_table + (long long)b * p.width;
-        for (int k = q.have + lane; k < q.want; k += 32)
-            row[k] = p.ring[(int)(((long long)head + q.base + (k - q.have)) % p.pool)];
-        if (q.flags & 16)
-            for (int k = lane; k < q.have; k += 32)
-                if (q.base + k < released) p.ring[(int)(((long long)head + count + q.base + k) % p.pool)] = row[k];
+        // both indices stay below twice the pool: new blocks are among `count`, released ones among the rest
+#pragma unroll 4
+        for (int k = q.have + lane; k < q.want; k += 32) row[k] = p.ring[wrap(head + q.base + (k - q.have))];
+        if (q.flags & 16) {
+            const int n = min(q.have, released - q.base);
+            for (int k = lane; k < n; k += 4 * 32) {             // four loads on their way at a time
+                int block[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (k + 32 * i < n) block[i] = row[k + 32 * i];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (k + 32 * i < n) p.ring[wrap(wrap(head + count) + q.base + k + 32 * i)] = block[i];
+            }
+        }
     }
     // rows
     const int live = first[p.seqs];
@@ -162,7 +173,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanParams 
             if ((q.flags & 15) == PLAN_OK) {
                 const int k = pos >> p.shift;
                 const int block = k < q.have ? p.block_table[(long long)lo * p.width + k]
-                                             : p.ring[(int)(((long long)head + q.base + (k - q.have)) % p.pool)];
+                                             : p.ring[wrap(head + q.base + (k - q.have))];
                 if (block >= 0 && block < p.pool) slot = (block << p.shift) + (pos & (bs - 1));
             }
         }
