@@ -11,13 +11,16 @@
 //
 // Roles of the warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread is a row: TMEM lane), then kTcaConv for K codes ->
 // operand and kTcaConv for V (loaded one step ahead, their blocks and scales two), the last issues the products.  The two tiles alternate: while one is in its softmax
-// the tensor cores work for the other.  The running maximum moves only when a score exceeds it by more than kTcaSlack
+// the tensor cores work for the other.  The running maximum moves only when a score exceeds it by more than a slack
 // (then the row's O is rescaled in TMEM), as does the reference of the V scales.
 // Operands stand in the canonical K-major layout without swizzle: core matrices of 8 rows x 16 bytes, 128 bytes apart along
 // the contraction; both store patterns below are free of bank conflicts.
 //
 // What bounds it: per step and SM 2048 clocks of tensor time, the same of exponentials (16 per clock) and the same of
 // shared-memory traffic; P is rounded to fp16 like the outputs.
+//
+// With fp32 inputs or outputs (SPLIT) an item is one tile of 128 rows: its queries are two fp16 terms in the places of the two
+// tiles, its weights two terms with the second in the columns of the second tile's scores, and every product is done for both.
 //
 // With few items the keys are cut into `splits` ranges of steps; a CTA then leaves {max, sum, rows} in the workspace and
 // attn_tc_join_kernel adds the ranges in order.
@@ -30,14 +33,12 @@
 
 namespace ztq {
 
-constexpr int kTcaRows = 256, kTcaKeys = 128;
+constexpr int kTcaKeys = 128;
+__host__ __device__ constexpr int tca_rows(bool split) { return split ? 128 : 256; }     // rows of an item
 constexpr int kTcaConv = 4;                      // warps that convert K, and as many V (two each would leave every thread 128 registers: 596 against 589 us for a chunk of 4096 over 8192)
 constexpr int kTcaGroups = 8 / kTcaConv;         // groups of 16 keys that each of them takes
 constexpr int kTcaMma = 8 + 2 * kTcaConv;
 constexpr int kTcaThreads = 32 * (kTcaMma + 1);
-constexpr float kTcaLift = 4.f, kTcaSlack = 8.f;  // with kTcaScaleSlack and the scales' significands below 2: P < 2^15
-constexpr int kTcaScaleSlack = 2;
-static_assert(kTcaLift + kTcaSlack + kTcaScaleSlack + 1 < 16, "P stays below 2^15");
 
 struct __align__(16) TcaInfo {                  // one step's factors, by groups of 16 keys
     float ks[8], vs[8];                         // |K scale|; V scale / 2^vexp, 0 where it is not finite
@@ -52,27 +53,27 @@ struct TcaShared {
 };
 template <int D>
 __host__ __device__ constexpr int tca_smem() {
-    const int n = kTcaRows * D * 2 + 4 * kTcaKeys * D * 2 + 1024;
+    const int n = 256 * D * 2 + 4 * kTcaKeys * D * 2 + 1024;
     return n < 120 * 1024 ? 120 * 1024 : n;     // one CTA per SM: it holds all of TMEM
 }
 
 struct TcaParams {
     AttnParams a;
-    int splits;
-    float* parts;                               // [item][split][256][D + 2]
+    int splits, rows;                           // rows of an item
+    float* parts;                               // [item][split][rows][D + 2]
 };
 
 struct TcaItem {
     int b, r0, r1, h, lo, hi;
     AttnSeq s;
 };
-// upto[b]: row pairs of sequences 0 .. b
-__device__ __forceinline__ void tca_scan(const AttnParams& p, int* upto, int* part) {
+// upto[b]: items of sequences 0 .. b for one kv head
+__device__ __forceinline__ void tca_scan(const AttnParams& p, int tile, int* upto, int* part) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     int before = 0;
     for (int b0 = 0; b0 < p.seqs; b0 += blockDim.x) {
         const int b = b0 + threadIdx.x;
-        int v = b < p.seqs ? (attn_seq(p, b).rows(p.group) + kTcaRows - 1) / kTcaRows : 0;
+        int v = b < p.seqs ? (attn_seq(p, b).rows(p.group) + tile - 1) / tile : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -93,7 +94,7 @@ __device__ __forceinline__ void tca_scan(const AttnParams& p, int* upto, int* pa
 }
 // Item i, or false behind the last.  Within a sequence the items with most keys come first: the hardware deals CTAs in
 // order, so the short ones fill the end.
-__device__ __forceinline__ bool tca_item(const AttnParams& p, const int* upto, long long i, TcaItem& it) {
+__device__ __forceinline__ bool tca_item(const AttnParams& p, int tile, const int* upto, long long i, TcaItem& it) {
     const int pair = (int)(i / p.kv_heads);
     it.h = (int)(i % p.kv_heads);
     if (pair >= upto[p.seqs - 1]) return false;
@@ -105,8 +106,8 @@ __device__ __forceinline__ bool tca_item(const AttnParams& p, const int* upto, l
     it.b = lo;
     it.s = attn_seq(p, lo);
     const int rows = it.s.rows(p.group);
-    it.r0 = (upto[lo] - 1 - pair) * kTcaRows;
-    it.r1 = min(it.r0 + kTcaRows, rows);
+    it.r0 = (upto[lo] - 1 - pair) * tile;
+    it.r1 = min(it.r0 + tile, rows);
     attn_span(p, it.s, it.r0, it.r1, it.lo, it.hi);
     return true;
 }
@@ -146,7 +147,7 @@ __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sy
 
 __device__ __forceinline__ uint32_t turned(uint32_t x, bool plus) { return plus ? unbias(x) : unbias(x) ^ 0x80008000u; }
 
-template <int D>
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams tp) {
     constexpr int CG = D / 8;                               // 16-byte columns of a K-major row of D
     constexpr int QB = 128 * D * 2, KB = kTcaKeys * D * 2;  // bytes of a tile of Q, of a K or V operand
@@ -163,14 +164,14 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
     grid_dep_wait();
     // the scan's scratch lies where the operands will be
     int* upto = reinterpret_cast<int*>(sk);
-    tca_scan(p, upto, reinterpret_cast<int*>(sv));
+    tca_scan(p, tca_rows(SPLIT), upto, reinterpret_cast<int*>(sv));
     TcaItem it;
-    const bool mine = tca_item(p, upto, blockIdx.x, it);
+    const bool mine = tca_item(p, tca_rows(SPLIT), upto, blockIdx.x, it);
     __syncthreads();
     if (!mine) return;
     const int kt_lo = it.lo / kTcaKeys, kt_all = max(0, (it.hi + kTcaKeys - 1) / kTcaKeys - kt_lo);
     const int kt0 = kt_lo + (int)((long long)kt_all * blockIdx.y / tp.splits), kt1 = kt_lo + (int)((long long)kt_all * (blockIdx.y + 1) / tp.splits);
-    const int n = kt1 - kt0, rows = it.r1 - it.r0, tiles = rows > 128 ? 2 : 1;
+    const int n = kt1 - kt0, rows = it.r1 - it.r0, tiles = !SPLIT && rows > 128 ? 2 : 1;
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -188,21 +189,35 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
     // queries: 16-byte pieces in K-major order, a phase of eight lanes writes eight rows of one column
     for (int i = tid; i < tiles * 128 * CG; i += kTcaThreads) {
         const int r = (i & 7) + (i >> 3) / CG * 8, col = (i >> 3) % CG, row = it.r0 + r;
-        uint4 v = make_uint4(0, 0, 0, 0);
+        uint4 v = make_uint4(0, 0, 0, 0), rest = v;
         if (row < it.r1) {
-            const __half* src = static_cast<const __half*>(p.q) + (it.s.first + row / p.group) * p.q_token + (long long)(it.h * p.group + row % p.group) * p.q_head + 8 * col;
-            if (p.vec) {
+            const long long at = (it.s.first + row / p.group) * p.q_token + (long long)(it.h * p.group + row % p.group) * p.q_head + 8 * col;
+            if (SPLIT && p.x_f32) {
+                const float* src = static_cast<const float*>(p.q) + at;
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = src[k];
+                v = make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+                rest = make_uint4(pack_rest(x[0], x[1], v.x), pack_rest(x[2], x[3], v.y), pack_rest(x[4], x[5], v.z), pack_rest(x[6], x[7], v.w));
+            } else if (p.vec) {
+                const __half* src = static_cast<const __half*>(p.q) + at;
                 const uint2 a = *reinterpret_cast<const uint2*>(src), b = *reinterpret_cast<const uint2*>(src + 4);
                 v = make_uint4(a.x, a.y, b.x, b.y);
             } else {
+                const __half* src = static_cast<const __half*>(p.q) + at;
                 uint32_t w[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) w[k] = (uint32_t)__half_as_ushort(src[2 * k]) | (uint32_t)__half_as_ushort(src[2 * k + 1]) << 16;
                 v = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            if (p.scale_log2 < 0) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }   // scores use |scale|
+            if (p.scale_log2 < 0) {                             // scores use |scale|
+                v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u;
+                rest.x ^= 0x80008000u; rest.y ^= 0x80008000u; rest.z ^= 0x80008000u; rest.w ^= 0x80008000u;
+            }
         }
-        *reinterpret_cast<uint4*>(sq + (r >> 3) * (CG * 128) + col * 128 + (r & 7) * 16) = v;
+        uint8_t* dst = sq + (r >> 3) * (CG * 128) + col * 128 + (r & 7) * 16;
+        *reinterpret_cast<uint4*>(dst) = v;
+        if constexpr (SPLIT) *reinterpret_cast<uint4*>(dst + QB) = rest;
     }
     proxy_fence_async();
     tc_fence_before();
@@ -355,6 +370,11 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                 const uint64_t a = tc_smem_desc(sq + t * QB, 128, CG * 128), b = tc_smem_desc(sk + (i & 1) * KB, 128, CG * 128);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) tc_mma_f16(tmem + kS + 128 * t, a + 16 * k, b + 16 * k, id_s, k > 0);
+                if constexpr (SPLIT) {
+                    const uint64_t rest = tc_smem_desc(sq + QB, 128, CG * 128);
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) tc_mma_f16(tmem + kS, rest + 16 * k, b + 16 * k, id_s, 1);
+                }
                 tc_commit(&sh.s_full[t]);
             };
             if (n > 0 && wait(&sh.k_full[0], 0)) {
@@ -371,6 +391,10 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                     const uint64_t b = tc_smem_desc(sv + (i & 1) * KB, 128, kTcaKeys / 8 * 128);
 #pragma unroll
                     for (int k = 0; k < kTcaKeys / 16; ++k) tc_mma_f16_ta(tmem + kO + D * t, tmem + kS + 128 * t + 8 * k, b + 16 * k, id_o, i > 0 || k > 0);
+                    if constexpr (SPLIT) {
+#pragma unroll
+                        for (int k = 0; k < kTcaKeys / 16; ++k) tc_mma_f16_ta(tmem + kO, tmem + kS + 128 + 8 * k, b + 16 * k, id_o, 1);
+                    }
                     if (t == tiles - 1) tc_commit(&sh.v_empty[i & 1]);
                     if (i + 1 < n) {
                         scores(t, i + 1);
@@ -436,7 +460,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                 fk[c] = info.ks[c] * scale;
                 top = tops[c] != -INFINITY ? fmaxf(top, tops[c] * fk[c]) : top;         // -inf may meet a factor of 0
             }
-            const bool grows = top > m + kTcaSlack, scale_grows = info.vexp > vrun + kTcaScaleSlack;
+            const bool grows = top > m + attn_slack(SPLIT), scale_grows = info.vexp > vrun + kAttnScaleSlack;
             if (__any_sync(0xffffffffu, grows) || scale_grows) {
                 const float m_new = fmaxf(m, top);
                 float fix = m == -INFINITY ? 0.f : ex2(m - m_new);
@@ -461,7 +485,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                 }
                 m = m_new;
             }
-            const float m_safe = m == -INFINITY ? 0.f : m, shift = kTcaLift + (float)max(info.vexp - vrun, -100) - m_safe;
+            const float m_safe = m == -INFINITY ? 0.f : m, shift = attn_lift(SPLIT) + (float)max(info.vexp - vrun, -100) - m_safe;
             f2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};
             float fv[8];
 #pragma unroll
@@ -470,6 +494,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                 scores([&](int c, const uint32_t (&r)[16]) {
                     const float f = fk[c], v = fv[c];
                     uint32_t u[8];
+                    [[maybe_unused]] uint32_t rest[SPLIT ? 8 : 1];
 #pragma unroll
                     for (int k = 0; k < 16; k += 2) {
                         const f2 x = ffma2(f2{__uint_as_float(r[k]), __uint_as_float(r[k + 1])}, f2{f, f}, f2{shift, shift});
@@ -481,8 +506,10 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                         sums[k >> 1 & 1] = fadd2(sums[k >> 1 & 1], f2{e0, e1});
                         const f2 w = ffma2(f2{e0, e1}, f2{v, v}, f2{0.f, 0.f});
                         u[k >> 1] = pack_half2(w.x, w.y);
+                        if constexpr (SPLIT) rest[k >> 1] = pack_rest(w.x, w.y, u[k >> 1]);
                     }
                     tc_st8(s_at + 8 * c, u);                    // over scores that were read
+                    if constexpr (SPLIT) tc_st8(s_at + 128 + 8 * c, rest);
                 });
             };
             if (edge) weights(std::true_type());
@@ -499,8 +526,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
         // ---- the row's output, or its part
         const float vref = n > 0 && vrun > -1000 ? ex2((float)vrun) : 0.f;
         const float inv = l > 0.f || l != l ? vref / l : 0.f;
-        float* part = tp.parts + (((long long)blockIdx.x * tp.splits + blockIdx.y) * kTcaRows + (r - it.r0)) * (D + 2);
-        const long long to = live ? (it.s.first + r / p.group) * p.y_token + (long long)(it.h * p.group + r % p.group) * p.y_head : 0;
+        float* part = tp.parts + (((long long)blockIdx.x * tp.splits + blockIdx.y) * tca_rows(SPLIT) + (r - it.r0)) * (D + 2);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
             float o[32];
@@ -514,15 +540,12 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) *reinterpret_cast<float2*>(part + 32 * c + k) = make_float2(o[k] * vref, o[k + 1] * vref);
             } else {
-                __half* y = static_cast<__half*>(p.y) + to + 32 * c;
-                if (p.y_wide) {
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8)
-                        *reinterpret_cast<uint4*>(y + k) = make_uint4(pack_half2(o[k] * inv, o[k + 1] * inv), pack_half2(o[k + 2] * inv, o[k + 3] * inv),
-                                                                      pack_half2(o[k + 4] * inv, o[k + 5] * inv), pack_half2(o[k + 6] * inv, o[k + 7] * inv));
-                } else {
+                for (int k = 0; k < 32; k += 8) {
+                    float v[8];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) y[k] = __float2half_rn(o[k] * inv);
+                    for (int e = 0; e < 8; ++e) v[e] = o[k + e] * inv;
+                    attn_store8(p, it.s, r, it.h, 32 * c + k, v);
                 }
             }
         }
@@ -544,13 +567,13 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const TcaParams tp) {
     const AttnParams& p = tp.a;
     grid_dep_launch();
     grid_dep_wait();
-    tca_scan(p, tca_upto, part);
+    tca_scan(p, tp.rows, tca_upto, part);
     TcaItem it;
-    if (!tca_item(p, tca_upto, blockIdx.x, it)) return;
+    if (!tca_item(p, tp.rows, tca_upto, blockIdx.x, it)) return;
     const int lane = threadIdx.x & 31, r = it.r0 + blockIdx.y * 8 + (threadIdx.x >> 5);
     if (r >= it.r1) return;
     float top = -INFINITY;
-    auto row_of = [&](int u) { return tp.parts + (((long long)blockIdx.x * tp.splits + u) * kTcaRows + (r - it.r0)) * (D + 2); };
+    auto row_of = [&](int u) { return tp.parts + (((long long)blockIdx.x * tp.splits + u) * tp.rows + (r - it.r0)) * (D + 2); };
     for (int u = 0; u < tp.splits; ++u) top = fmaxf(top, row_of(u)[D]);
     float sum = 0.f, v[D / 32] = {};
     for (int u = 0; u < tp.splits; ++u) {

@@ -52,7 +52,7 @@ static cudaError_t launch_dim(const AttnParams& p, int nt, bool split, int sms, 
     return split ? launch_rows<D, 1, true>(p, sms, stream, pdl) : launch_rows<D, 1, false>(p, sms, stream, pdl);
 }
 
-// Prompts: sequences with more than kTcMinRows rows per kv head go to the tensor-core kernel (fp16, heads of 64 and 128).
+// Prompts: sequences with more than kTcMinRows rows per kv head go to the tensor-core kernel (heads of 64 and 128).
 // With few sequences all of them do: a launch of its own for those with few rows would cost more than their 256-row items
 // (three sequences of 91, 26 and 91 tokens: 58 us with both kernels and their joins, 33 with one).
 constexpr int kTcMinRows = 64;
@@ -63,34 +63,35 @@ struct TcPlan {
     bool all = false;             // takes every sequence
     size_t bytes = 0;             // of its workspace
 };
-static TcPlan tc_plan(int tokens, int sequences, long long most_rows, int group, int kv_heads, int head_dim, int sms) {
+static TcPlan tc_plan(int tokens, int sequences, long long most_rows, int group, int kv_heads, int head_dim, bool split, int sms) {
     TcPlan t;
     if (most_rows <= kTcMinRows || head_dim > 128) return t;
     t.all = sequences == 1 || (long long)sequences * kv_heads <= sms;
-    // an item is 256 rows of a sequence: full ones, and one begun by each sequence that is taken
-    const long long rows = (long long)tokens * group, full = rows / kTcaRows;
+    // items: full ones, and one begun by each sequence that is taken
+    const long long rows = (long long)tokens * group, full = rows / tca_rows(split);
     const long long begun = t.all ? sequences : std::min<long long>(sequences, rows / (kTcMinRows + 1) + 1);
     t.items = (full + begun) * kv_heads;
     // few items: cut their keys so that every SM has a CTA
     const long long few = (full > 0 ? full : 1) * kv_heads;
     if (few < sms) t.splits = (int)std::min<long long>(sms / few, 32);
-    if (t.splits > 1) t.bytes = (size_t)t.items * t.splits * kTcaRows * (head_dim + 2) * sizeof(float);
+    if (t.splits > 1) t.bytes = (size_t)t.items * t.splits * tca_rows(split) * (head_dim + 2) * sizeof(float);
     return t;
 }
 
-template <int D>
+template <int D, bool SPLIT>
 static cudaError_t launch_tc(const AttnParams& p, const TcPlan& plan, cudaStream_t stream, bool pdl) {
     TcaParams tp;
     tp.a = p;
     // a split is worth eight steps: the join takes as long as two
     tp.splits = (int)std::max<long long>(1, std::min<long long>(plan.splits, ((long long)p.width << p.shift) / (8 * kTcaKeys)));
+    tp.rows = tca_rows(SPLIT);
     tp.parts = p.parts;
     static std::atomic<unsigned> done{0};
-    auto kern = attn_tc_kernel<D>;
+    auto kern = attn_tc_kernel<D, SPLIT>;
     if (cudaError_t e = allow_smem(kern, done, tca_smem<D>())) return e;
     cudaError_t e = launch(kern, dim3((unsigned)plan.items, tp.splits), dim3(kTcaThreads), tca_smem<D>(), stream, pdl, tp);
     if (e != cudaSuccess) return e;
-    if (tp.splits > 1) e = launch(attn_tc_join_kernel<D>, dim3((unsigned)plan.items, kTcaRows / 8), dim3(256), p.seqs * sizeof(int), stream, pdl, tp);
+    if (tp.splits > 1) e = launch(attn_tc_join_kernel<D>, dim3((unsigned)plan.items, tp.rows / 8), dim3(256), p.seqs * sizeof(int), stream, pdl, tp);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -115,7 +116,7 @@ size_t ztq_attn_q8_workspace_bytes(int tokens, int sequences, int max_new, int q
     const long long rows = (long long)max_new * group;
     const int nt = attn_nt(head_dim, rows, false);
     return std::max((size_t)sms * 2 * 8 * nt * (head_dim + 2) * sizeof(float),
-                    tc_plan(tokens, sequences, rows, group, kv_heads, head_dim, sms).bytes);
+                    std::max(tc_plan(tokens, sequences, rows, group, kv_heads, head_dim, false, sms).bytes, tc_plan(tokens, sequences, rows, group, kv_heads, head_dim, true, sms).bytes));
 }
 
 cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_head, long long y_token, long long y_head, int tokens, int q_heads,
@@ -169,16 +170,15 @@ cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_h
     p.max_rows = 0x7fffffff;
     const bool split = p.x_f32 || p.y_f32, pdl = !(flags & ZTQ_NO_PDL);
     const int nt = attn_nt(dim, (long long)max_new * p.group, split);
-    if (!split) {
-        const TcPlan plan = tc_plan(tokens, sequences, (long long)max_new * p.group, p.group, p.kv_heads, dim, dev.sms);
-        if (plan.items > 0x7fffffff) return cudaErrorInvalidValue;
-        if (plan.items > 0) {
-            if (!plan.all) p.min_rows = kTcMinRows + 1;          // told apart on the device, where the lengths are
-            cudaError_t e = dim == 64 ? launch_tc<64>(p, plan, stream, pdl) : launch_tc<128>(p, plan, stream, pdl);
-            if (e != cudaSuccess || plan.all) return e;
-            p.min_rows = 1;
-            p.max_rows = kTcMinRows;
-        }
+    const TcPlan plan = tc_plan(tokens, sequences, (long long)max_new * p.group, p.group, p.kv_heads, dim, split, dev.sms);
+    if (plan.items > 0x7fffffff) return cudaErrorInvalidValue;
+    if (plan.items > 0) {
+        if (!plan.all) p.min_rows = kTcMinRows + 1;              // told apart on the device, where the lengths are
+        cudaError_t e = dim == 64 ? (split ? launch_tc<64, true>(p, plan, stream, pdl) : launch_tc<64, false>(p, plan, stream, pdl))
+                                  : (split ? launch_tc<128, true>(p, plan, stream, pdl) : launch_tc<128, false>(p, plan, stream, pdl));
+        if (e != cudaSuccess || plan.all) return e;
+        p.min_rows = 1;
+        p.max_rows = kTcMinRows;
     }
     return dim == 64 ? launch_dim<64>(p, nt, split, dev.sms, stream, pdl)
          : dim == 128 ? launch_dim<128>(p, nt, split, dev.sms, stream, pdl) : launch_dim<256>(p, nt, split, dev.sms, stream, pdl);
