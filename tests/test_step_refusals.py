@@ -79,6 +79,7 @@ def test_the_unchanged_calls_pass_the_checks(name):
 def test_workspace_of_impossible_sizes_is_zero():
     f = K.attn_q8_workspace_bytes
     assert f(4, 4, 1, 64, 8, 128) > 0
+    assert max(f(n * s, s, n, 64, 8, 128) for n in (1, 2, 9, 40, 1000) for s in (1, 2, 5, 18, 19, 64, 500, 4096)) <= 160 << 20
     for bad in ((-1, 4, 1, 64, 8, 128), (4, 0, 1, 64, 8, 128), (4, 4, 0, 64, 8, 128), (4, 4, 1, 63, 8, 128), (4, 4, 1, 64, 0, 128), (4, 4, 1, 64, 8, 100)):
         assert f(*bad) == 0
 

@@ -71,8 +71,9 @@ static TcPlan tc_plan(int tokens, int sequences, long long most_rows, int group,
     const long long rows = (long long)tokens * group, full = rows / tca_rows(split);
     const long long begun = t.all ? sequences : std::min<long long>(sequences, rows / (kTcMinRows + 1) + 1);
     t.items = (full + begun) * kv_heads;
-    // few items: cut their keys so that every SM has a CTA
-    const long long few = (full > 0 ? full : 1) * kv_heads;
+    // few items: cut their keys so that every SM has a CTA.  Half the begun ones are taken to be there: counting on fewer
+    // would make the workspace (items x splits) grow with the square of the sequences
+    const long long few = std::max(full, (begun + 1) / 2) * kv_heads;
     if (few < sms) t.splits = (int)std::min<long long>(sms / few, 32);
     if (t.splits > 1) t.bytes = (size_t)t.items * t.splits * tca_rows(split) * (head_dim + 2) * sizeof(float);
     return t;
