@@ -28,6 +28,9 @@
 //   A tile of 16 tokens lies in one block (block sizes are multiples of 16), so its scales are two scalars: sk goes into
 // the score's factor, sv over a running power of two into p.
 //
+// Measured: 64 sequences of 3000 to 12000 tokens, 64 / 8 heads of 128 (958 MB) 193 us = 4.96 TB/s, 160 with the arithmetic
+// left out; one sequence of 8192 tokens 18 us with the join, of which the copies and the arithmetic take 4.
+//
 // Work: an item is (sequence, tile of rows, kv head).  The steps of all items in order are dealt to the CTAs in equal
 // contiguous ranges, whatever the lengths, so a long sequence is split and short ones are packed.  A CTA that holds part of
 // an item leaves {max, sum, rows} in the workspace (at most two parts per CTA) and attn_join_kernel adds the parts in

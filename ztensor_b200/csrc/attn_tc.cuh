@@ -10,14 +10,16 @@
 // scores in the softmax, whose exponent's factor takes sk and whose weights take sv over a running power of two.
 //
 // Roles of the warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread is a row: TMEM lane), then kTcaConv for K codes ->
-// operand and kTcaConv for V (loaded one step ahead, their blocks and scales two), the last issues the products.  The two tiles alternate: while one is in its softmax
-// the tensor cores work for the other.  The running maximum moves only when a score exceeds it by more than a slack
+// operand and kTcaConv for V (loaded one step ahead, their blocks and scales two), the last issues the products.  The two
+// tiles alternate: while one is in its softmax the tensor cores work for the other.  The running maximum moves only when a score exceeds it by more than a slack
 // (then the row's O is rescaled in TMEM), as does the reference of the V scales.
 // Operands stand in the canonical K-major layout without swizzle: core matrices of 8 rows x 16 bytes, 128 bytes apart along
 // the contraction; both store patterns below are free of bank conflicts.
 //
-// What bounds it: per step and SM 2048 clocks of tensor time, the same of exponentials (16 per clock) and the same of
-// shared-memory traffic; P is rounded to fp16 like the outputs.
+// What bounds it: per step and SM there are 2048 clocks of tensor time, the same of exponentials (16 per clock) and the same of
+// shared-memory traffic, but the chain scores -> maximum -> weights -> products of two tiles overlaps them only in part: 4096
+// new tokens over 8192 keys, 32 / 8 heads of 128 take 589 us (700 TFLOP/s), the products alone 325, without the conversions
+// 434, without the exponentials 481.  P is rounded to fp16 like the outputs.
 //
 // With fp32 inputs or outputs (SPLIT) an item is one tile of 128 rows: its queries are two fp16 terms in the places of the two
 // tiles, its weights two terms with the second in the columns of the second tile's scores, and every product is done for both.
@@ -35,7 +37,7 @@ namespace ztq {
 
 constexpr int kTcaKeys = 128;
 __host__ __device__ constexpr int tca_rows(bool split) { return split ? 128 : 256; }     // rows of an item
-constexpr int kTcaConv = 4;                      // warps that convert K, and as many V (two each would leave every thread 128 registers: 596 against 589 us for a chunk of 4096 over 8192)
+constexpr int kTcaConv = 4;                      // warps that convert K, and as many V (two each leave 128 registers per thread: 596 against 589 us)
 constexpr int kTcaGroups = 8 / kTcaConv;         // groups of 16 keys that each of them takes
 constexpr int kTcaMma = 8 + 2 * kTcaConv;
 constexpr int kTcaThreads = 32 * (kTcaMma + 1);
