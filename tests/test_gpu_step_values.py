@@ -1,0 +1,153 @@
+"""Attention and the operators around it at values far from one: queries and scales of any size, blocks that a row does not see, refused sequences."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests import step_ref as R
+from tests import util as U
+from tests.test_gpu_step import DEV, FEW, HALF16, HALF32, MANY, MIXED, ONE, attn_case, dev, host, no_error
+from ztensor_b200 import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def a_clean_error_word():
+    K.device_error()
+
+
+def run(lens, cache, table, start, kv_len, q, y, scale, window=0, most=None):
+    most = most or max(1, max(a for _, a in lens))
+    ws = torch.full((K.attn_q8_workspace_bytes(q.shape[0], len(lens), most, q.shape[1], cache.kv_heads, cache.head_dim) // 4,), math.nan, device=DEV)
+    K.attn_q8(q, y, start, kv_len, table, cache, ws, most, scale, window)
+
+
+def check(lens, cache, table, q, y, scale, window=0, f32=False, rows=None):
+    """Every row against 64 bits.  The bound holds for values of any size, because each part of it is relative to what the row itself sees:
+      a score is an fp32 sum of D / 16 + 2 roundings, its query is held to 2^-22 of itself (fp32: two fp16 terms) or exactly, and an element far
+          below the row's largest to 2^-39 of that one (fp16's last step below 2^15);
+      a weight has fp16's half step, or that of two terms, and a few roundings of the exponential;
+      a weight times its V scale far below the row's largest such product ends at fp16's last half step, 2^-25, where the largest is held as 2^4
+          (fp32: 2^12) within a factor of 2^0.5;
+      sums over n keys take n / 16 more roundings of 2^-23; the output has its own half step."""
+    codes_k, codes_v, ks, vs = (host(t).astype(np.float64) for t in cache.tensors)
+    size, dim, group = cache.block_size, cache.head_dim, q.shape[1] // cache.kv_heads
+    got, qh, table = host(y), host(q), table.cpu().numpy()
+    row = 0
+    for b, (n, a) in enumerate(lens):
+        block, at = table[b][np.arange(n) // size], np.arange(n) % size
+        there = (block >= 0) & (block < cache.blocks)
+        block = np.where(there, block, 0)
+        for h in range(cache.kv_heads):
+            kk, cv, sv = codes_k[block, h, at] * ks[block, h][:, None], codes_v[block, h, at], vs[block, h]
+            for i in range(a):
+                if rows is not None and i not in rows:
+                    continue
+                pos = n - a + i
+                seen = there & (np.arange(n) <= pos) & (np.arange(n) > pos - window if window else True)
+                for g in range(h * group, (h + 1) * group):
+                    out = got[row + i, g]
+                    if not seen.any():
+                        assert (out == 0).all()
+                        continue
+                    x = qh[row + i, g]
+                    s = kk[seen] @ x * scale
+                    p = np.exp(s - s.max())
+                    p /= p.sum()
+                    w, c = p * sv[seen], cv[seen]
+                    ref, mean = w @ c, np.abs(w) @ np.abs(c)
+                    reach = abs(scale) * (np.abs(kk[seen]) @ np.abs(x)).max()
+                    far = abs(scale) * np.abs(kk[seen]).sum(1).max() * np.abs(x).max() * 2.0 ** -39 if f32 else 0.0
+                    score = (dim / 16 + 2) * 2 * HALF32 * reach + (2.0 ** -22 * reach if f32 else 0.0) + far
+                    weight = score + (4 * 2.0 ** -22 if f32 else HALF16) + (64 + seen.sum() / 8) * HALF32
+                    ends = 2.0 ** (-36.5 if f32 else -28.5) * np.abs(w).max() * np.abs(c).sum(0)
+                    tol = 2 * weight * mean + ends + (2.0 ** -126 if y.dtype is torch.float32 else HALF16 * np.abs(ref) + 2.0 ** -25)
+                    worst = np.abs(out - ref) / tol
+                    assert (worst <= 1).all(), (b, i, g, float(np.nanmax(worst)), out[:4], ref[:4])
+        row += a
+    assert (got[row:] == 0.5).all()
+
+
+# ------------------------------------------------------------------ fp32 queries of any size
+
+ROWS = [(200, 1), (77, 1), (33, 1)]                  # few rows per kv head
+PROMPT = [(300, 40), (90, 64)]
+
+
+@pytest.mark.parametrize("dim,lens", [(64, ROWS), (128, ROWS), (256, ROWS), (64, FEW), (256, PROMPT), (64, PROMPT), (128, PROMPT)])
+@pytest.mark.parametrize("size", [1e-30, 3e-8, 1e-5, 1e-3, 6e4, 1e6, 1e30])
+def test_fp32_queries_of_any_size(dim, lens, size):
+    """The keys' scales are as far the other way, so that the scores stay of order one."""
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(dim), lens, 2, 4, 16, dim, torch.float32)
+    q *= size
+    cache.tensors[2].mul_(2.0 ** -round(math.log2(size)))
+    run(lens, cache, table, start, kv_len, q, y, 1 / math.sqrt(dim))
+    check(lens, cache, table, q, y, 1 / math.sqrt(dim), f32=True)
+    no_error()
+
+
+@pytest.mark.parametrize("dim,lens", [(64, ROWS), (128, FEW), (256, FEW), (64, PROMPT), (128, PROMPT)])
+def test_fp32_rows_and_elements_of_different_sizes(dim, lens):
+    """Each row has a size of its own, and some have one element far above the others; rows of zeros and of subnormal numbers among them."""
+    rng = U.seeded(dim + 1)
+    cache, table, start, kv_len, q, y = attn_case(rng, lens, 2, 4, 32, dim, torch.float32)
+    x = host(q) * np.exp2(rng.integers(-40, 3, q.shape[:2]))[..., None]
+    x[::3, 1, dim // 3] *= 2.0 ** 20
+    x[::4, 2] = 0
+    x[::2, 3] *= 2.0 ** -110
+    q.copy_(dev(x))
+    run(lens, cache, table, start, kv_len, q, y, 0.1)
+    check(lens, cache, table, q, y, 0.1, f32=True)
+    no_error()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens", [ROWS, PROMPT], ids=["rows", "prompt"])
+def test_fp32_queries_that_are_not_finite(dim, lens):
+    """Such a row is NaN; the others are as without it."""
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(dim), lens, 2, 4, 16, dim, torch.float32)
+    q[1, 3, 5], q[0, 6, 1] = math.inf, math.nan
+    run(lens, cache, table, start, kv_len, q, y, 0.1)
+    assert torch.isnan(y[1, 3]).all() and torch.isnan(y[0, 6]).all() and not torch.isnan(y[2:]).any()
+    got = y.clone()
+    q[1, 3, 5], q[0, 6, 1] = 0.0, 0.0
+    y.fill_(0.5)
+    run(lens, cache, table, start, kv_len, q, y, 0.1)
+    check(lens, cache, table, q, y, 0.1, f32=True)
+    got[1, 3], got[0, 6] = y[1, 3], y[0, 6]
+    assert torch.equal(got, y)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("x32,y32", [(True, True), (True, False), (False, True)])
+@pytest.mark.parametrize("lens,window", [([(3000, 260)], 0), ([(5000, 150), (3, 2), (2100, 90)], 0), ([(4100, 33)], 2500)])
+def test_fp32_prompts_with_their_keys_in_ranges(dim, x32, y32, lens, window):
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(7), lens, 1, 4, 64, dim, torch.float32 if x32 else torch.float16)
+    y = torch.full(q.shape, 0.5, dtype=torch.float32 if y32 else torch.float16, device=DEV)
+    run(lens, cache, table, start, kv_len, q, y, 0.05, window)
+    check(lens, cache, table, q, y, 0.05, window, f32=True, rows=range(0, 300, 13))
+    no_error()
+
+
+@pytest.mark.parametrize("heads,group,dim", [(4, 4, 64), (4, 3, 128), (4, 2, 256)])
+def test_fp32_batches_that_two_kernels_share(heads, group, dim):
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(9), MIXED, heads, group, 64, dim, torch.float32)
+    run(MIXED, cache, table, start, kv_len, q, y, 1 / math.sqrt(dim))
+    check(MIXED, cache, table, q, y, 1 / math.sqrt(dim), f32=True, rows=range(0, 80, 17))
+    no_error()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 3, 50])
+def test_fp32_scales_of_any_kind(new, dim):
+    lens = [(300, new), (50 + new, new)]
+    rng = U.seeded(13)
+    cache, table, start, kv_len, q, y = attn_case(rng, lens, 2, 4, 16, dim, torch.float32)
+    for t in cache.tensors[2:]:
+        t.copy_(dev((rng.uniform(0.5, 1.5, t.shape) * np.exp2(rng.integers(-16, -4, t.shape)) * rng.choice([1, 1, 1, -1, 0], t.shape)).astype(np.float32)))
+    for scale in (0.1, -0.1, 0.0):
+        run(lens, cache, table, start, kv_len, q, y, scale)
+        check(lens, cache, table, q, y, scale, f32=True)
+    no_error()

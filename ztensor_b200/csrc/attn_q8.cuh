@@ -24,7 +24,8 @@
 // exponent (one vote per 16 tokens instead of a reduction); p = 2^(s - m + 4) then stays inside fp16 and ends at 2^-28 of the
 // largest weight.  Scores, maxima, sums and accumulators are fp32; p is rounded to
 // fp16 for the second product (relative 2^-11, against fp16 outputs with the same step).  With fp32 inputs or outputs
-// (SPLIT) q and p go in as two fp16 terms each, 22 bits.
+// (SPLIT) q and p go in as two fp16 terms each, 22 bits; a row of fp32 queries is first brought near the upper end of fp16's
+// range by a power of two, which its scores are divided by.
 //   A tile of 16 tokens lies in one block (block sizes are multiples of 16), so its scales are two scalars: sk goes into
 // the score's factor, sv over a running power of two into p.
 //
@@ -126,6 +127,10 @@ __device__ __forceinline__ uint32_t unbias(uint32_t x) {
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// The power of two that brings a row whose largest element is `top` to [2^14, 2^15), where two fp16 terms hold 22 bits of every element
+// down to 2^-17 of the largest, and the others to 2^-39 of that (a row below 2^-112 stays below, and its subnormal numbers are exact).
+__device__ __forceinline__ float attn_up(float top) { return __uint_as_float(min(127 + 14 + 127 - (__float_as_uint(top) >> 23), 253u) << 23); }
+__device__ __forceinline__ float attn_down(float up) { return __uint_as_float((254u << 23) - __float_as_uint(up)); }      // its reciprocal
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -374,35 +379,53 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
 
         // the item's queries as B fragments; columns are the rows r0 + 8 t + g
         uint32_t qh[NT][KS][2], ql[SPLIT ? NT : 1][KS][2];
+        [[maybe_unused]] float down[SPLIT ? NT : 1][2];         // fp32 queries: what the scores of rows 2c, 2c + 1 are multiplied by
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int r = it.r0 + 8 * t + g;
             const bool live = r < it.r1;
-            const long long at = live ? (s.first + r / p.group) * p.q_token + (long long)(head + r % p.group) * p.q_head : 0;
+            const long long at = (live ? (s.first + r / p.group) * p.q_token + (long long)(head + r % p.group) * p.q_head : 0) + 16 * c;
+            if constexpr (SPLIT) {
+                float up = 1.f;
+                if (p.x_f32) {
+                    float v[KS][4], top = 0.f;
+#pragma unroll
+                    for (int j = 0; j < KS; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            v[j][i] = live ? static_cast<const float*>(p.q)[at + 64 * (j / 4) + 4 * (j % 4) + i] : 0.f;
+                            top = fmaxf(top, fabsf(v[j][i]));
+                        }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));        // the row's other pieces
+                    up = attn_up(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)));
+#pragma unroll
+                    for (int j = 0; j < KS; ++j)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float x = v[j][2 * i] * up, y = v[j][2 * i + 1] * up;
+                            qh[t][j][i] = pack_half2(x, y);
+                            ql[t][j][i] = pack_rest(x, y, qh[t][j][i]);
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) down[t][i] = attn_down(__shfl_sync(0xffffffffu, up, 4 * (2 * c + i)));
+                if (p.x_f32) continue;
+            }
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
-                const long long d0 = at + 64 * (j / 4) + 16 * c + 4 * (j % 4);
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
+                const long long d0 = at + 64 * (j / 4) + 4 * (j % 4);
                 uint2 u = make_uint2(0, 0);
                 if (live) {
-                    if (p.x_f32) {
-                        const float* f = static_cast<const float*>(p.q) + d0;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = f[i];
-                    } else if (p.vec) {
+                    if (p.vec) {
                         u = *reinterpret_cast<const uint2*>(static_cast<const __half*>(p.q) + d0);
                     } else {
                         const unsigned short* f = static_cast<const unsigned short*>(p.q) + d0;
                         u = make_uint2(f[0] | (uint32_t)f[1] << 16, f[2] | (uint32_t)f[3] << 16);
                     }
                 }
-                if constexpr (SPLIT) {
-                    if (p.x_f32) u = make_uint2(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]));
-                    ql[t][j][0] = p.x_f32 ? pack_rest(v[0], v[1], u.x) : 0u;
-                    ql[t][j][1] = p.x_f32 ? pack_rest(v[2], v[3], u.y) : 0u;
-                }
                 qh[t][j][0] = u.x;
                 qh[t][j][1] = u.y;
+                if constexpr (SPLIT) ql[t][j][0] = ql[t][j][1] = 0u;
             }
         }
 
@@ -479,7 +502,7 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    sc[t][i] = (sc[t][i] + sd[t][i]) * f;
+                    sc[t][i] = (sc[t][i] + sd[t][i]) * (SPLIT ? f * down[SPLIT ? t : 0][i & 1] : f);
                     if (!whole_tile) {
                         const int key = tok + tau + 8 * (i >> 1), z = last[t][i & 1];
                         const bool seen = !hidden && key <= z && (p.window <= 0 || key > z - p.window);

@@ -21,8 +21,8 @@
 // new tokens over 8192 keys, 32 / 8 heads of 128 take 589 us (700 TFLOP/s), the products alone 325, without the conversions
 // 434, without the exponentials 481.  P is rounded to fp16 like the outputs.
 //
-// With fp32 inputs or outputs (SPLIT) an item is one tile of 128 rows: its queries are two fp16 terms in the places of the two
-// tiles, its weights two terms with the second in the columns of the second tile's scores, and every product is done for both.
+// With fp32 inputs or outputs (SPLIT) an item is one tile of 128 rows: its queries are two fp16 terms (of the row times a power of two,
+// which its scores are divided by) in the places of the two tiles, its weights two terms with the second in the columns of the second tile's scores, and every product is done for both.
 //
 // With few items the keys are cut into `splits` ranges of steps; a CTA then leaves {max, sum, rows} in the workspace and
 // attn_tc_join_kernel adds the ranges in order.
@@ -52,7 +52,9 @@ struct TcaShared {
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], info_full[4];
     TcaInfo info[4];
     uint32_t tmem;
+    float down[128];                            // fp32 queries: what a row's scores are multiplied by
 };
+static_assert(sizeof(TcaShared) <= 1024, "the end of tca_smem");
 template <int D>
 __host__ __device__ constexpr int tca_smem() {
     const int n = 256 * D * 2 + 4 * kTcaKeys * D * 2 + 1024;
@@ -188,38 +190,60 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // queries: 16-byte pieces in K-major order, a phase of eight lanes writes eight rows of one column
-    for (int i = tid; i < tiles * 128 * CG; i += kTcaThreads) {
-        const int r = (i & 7) + (i >> 3) / CG * 8, col = (i >> 3) % CG, row = it.r0 + r;
-        uint4 v = make_uint4(0, 0, 0, 0), rest = v;
-        if (row < it.r1) {
-            const long long at = (it.s.first + row / p.group) * p.q_token + (long long)(it.h * p.group + row % p.group) * p.q_head + 8 * col;
-            if (SPLIT && p.x_f32) {
-                const float* src = static_cast<const float*>(p.q) + at;
-                float x[8];
+    // queries: 16-byte pieces in K-major order, a phase of eight lanes writes eight rows of one column; scores use |scale|
+    auto query_at = [&](int row) { return (it.s.first + row / p.group) * p.q_token + (long long)(it.h * p.group + row % p.group) * p.q_head; };
+    auto place = [&](int r, int col) { return sq + (r >> 3) * (CG * 128) + col * 128 + (r & 7) * 16; };
+    if (SPLIT && p.x_f32) {
+        // a warp takes eight rows: a lane a row's columns lane / 8 + 4 j
+        for (int r = 8 * warp + (lane & 7); r < 128; r += kTcaThreads / 4) {
+            const int row = it.r0 + r;
+            float x[CG / 4][8], top = 0.f;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = src[k];
-                v = make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
-                rest = make_uint4(pack_rest(x[0], x[1], v.x), pack_rest(x[2], x[3], v.y), pack_rest(x[4], x[5], v.z), pack_rest(x[6], x[7], v.w));
-            } else if (p.vec) {
-                const __half* src = static_cast<const __half*>(p.q) + at;
-                const uint2 a = *reinterpret_cast<const uint2*>(src), b = *reinterpret_cast<const uint2*>(src + 4);
-                v = make_uint4(a.x, a.y, b.x, b.y);
-            } else {
-                const __half* src = static_cast<const __half*>(p.q) + at;
-                uint32_t w[4];
+            for (int j = 0; j < CG / 4; ++j)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) w[k] = (uint32_t)__half_as_ushort(src[2 * k]) | (uint32_t)__half_as_ushort(src[2 * k + 1]) << 16;
-                v = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-            if (p.scale_log2 < 0) {                             // scores use |scale|
-                v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u;
-                rest.x ^= 0x80008000u; rest.y ^= 0x80008000u; rest.z ^= 0x80008000u; rest.w ^= 0x80008000u;
+                for (int k = 0; k < 8; ++k) {
+                    x[j][k] = row < it.r1 ? static_cast<const float*>(p.q)[query_at(row) + 8 * (4 * j + (lane >> 3)) + k] : 0.f;
+                    top = fmaxf(top, fabsf(x[j][k]));
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            float up = attn_up(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)));
+            if (lane < 8) sh.down[r] = attn_down(up);
+            if (p.scale_log2 < 0) up = -up;
+#pragma unroll
+            for (int j = 0; j < CG / 4; ++j) {
+                uint32_t v[4], rest[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float a = x[j][2 * k] * up, b = x[j][2 * k + 1] * up;
+                    v[k] = pack_half2(a, b);
+                    rest[k] = pack_rest(a, b, v[k]);
+                }
+                uint8_t* dst = place(r, 4 * j + (lane >> 3));
+                *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<uint4*>(dst + QB) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
             }
         }
-        uint8_t* dst = sq + (r >> 3) * (CG * 128) + col * 128 + (r & 7) * 16;
-        *reinterpret_cast<uint4*>(dst) = v;
-        if constexpr (SPLIT) *reinterpret_cast<uint4*>(dst + QB) = rest;
+    } else {
+        for (int i = tid; i < tiles * 128 * CG; i += kTcaThreads) {
+            const int r = (i & 7) + (i >> 3) / CG * 8, col = (i >> 3) % CG, row = it.r0 + r;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (row < it.r1) {
+                const __half* src = static_cast<const __half*>(p.q) + query_at(row) + 8 * col;
+                if (p.vec) {
+                    const uint2 a = *reinterpret_cast<const uint2*>(src), b = *reinterpret_cast<const uint2*>(src + 4);
+                    v = make_uint4(a.x, a.y, b.x, b.y);
+                } else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[k] = (uint32_t)__half_as_ushort(src[2 * k]) | (uint32_t)__half_as_ushort(src[2 * k + 1]) << 16;
+                    v = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                if (p.scale_log2 < 0) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
+            }
+            *reinterpret_cast<uint4*>(place(r, col)) = v;
+            if constexpr (SPLIT) *reinterpret_cast<uint4*>(place(r, col) + QB) = make_uint4(0, 0, 0, 0);
+            if (SPLIT && col == 0) sh.down[r] = 1.f;
+        }
     }
     proxy_fence_async();
     tc_fence_before();
@@ -415,7 +439,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
         const int base = it.s.len - it.s.fresh;
         const int z = live ? min(base + r / p.group, it.s.len - 1) : -1;    // last key the row sees
         const int z_lo = p.window > 0 ? z - p.window : -1;                  // the last one in front of those it sees
-        const float scale = fabsf(p.scale_log2);
+        const float scale = fabsf(p.scale_log2), down = SPLIT ? sh.down[r - it.r0] : 1.f;
         float m = -INFINITY, l = 0.f;
         int vrun = -1000;
         for (int i = 0; i < n; ++i) {
@@ -460,6 +484,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
                 fk[c] = info.ks[c] * scale;
+                if constexpr (SPLIT) fk[c] *= down;
                 top = tops[c] != -INFINITY ? fmaxf(top, tops[c] * fk[c]) : top;         // -inf may meet a factor of 0
             }
             const bool grows = top > m + attn_slack(SPLIT), scale_grows = info.vexp > vrun + kAttnScaleSlack;
