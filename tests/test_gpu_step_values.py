@@ -151,3 +151,31 @@ def test_fp32_scales_of_any_kind(new, dim):
         run(lens, cache, table, start, kv_len, q, y, scale)
         check(lens, cache, table, q, y, scale, f32=True)
     no_error()
+
+
+# ------------------------------------------------------------------ V scales far apart
+
+@pytest.mark.parametrize("f32,small", [(False, -16), (True, -16), (True, -60)])
+@pytest.mark.parametrize("dim,new", [(64, 1), (64, 40), (128, 40), (128, 3), (256, 20)])
+@pytest.mark.parametrize("where", [0, 1, 2])
+def test_steps_without_v_scales(f32, small, dim, new, where):
+    """All V scales of 128 tokens are zero, in front of, between or behind tokens of small ones."""
+    lens = [(128 * 3, new)]
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(dim), lens, 2, 4, 16, dim, torch.float32 if f32 else torch.float16)
+    cache.tensors[3].mul_(2.0 ** (small + 7))
+    cache.tensors[3][table[0, 8 * where:8 * where + 8].long()] = 0.0
+    run(lens, cache, table, start, kv_len, q, y, 0.05)
+    check(lens, cache, table, q, y, 0.05, f32=f32)
+    no_error()
+
+
+@pytest.mark.parametrize("f32,small", [(False, -16), (True, -60)])
+@pytest.mark.parametrize("dim,new", [(64, 1), (64, 40), (128, 40)])
+def test_steps_without_blocks(f32, small, dim, new):
+    lens = [(128 * 3, new)]
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(dim), lens, 2, 4, 16, dim, torch.float32 if f32 else torch.float16)
+    cache.tensors[3].mul_(2.0 ** (small + 7))
+    table[0, 8:16] = -1
+    run(lens, cache, table, start, kv_len, q, y, 0.05)
+    check(lens, cache, table, q, y, 0.05, f32=f32)
+    assert K.device_error() == 7

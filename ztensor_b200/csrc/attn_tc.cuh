@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                 uint32_t top = fine ? __float_as_uint(fabsf(sc)) >> 23 : 0u;
 #pragma unroll
                 for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const int vexp = top ? min(max((int)top - 127, -120), 120) : 0;
+                const int vexp = min(max((int)top - 127, -120), 120);       // -120 without any: the reference stays where real scales put it
                 const uint32_t bad = __ballot_sync(0xffffffffu, blk >= 0 && !fine) & 255u;
                 if (lane < 8) f.vs[lane] = fine ? sc * __uint_as_float((uint32_t)(127 - vexp) << 23) : 0.f;
                 if (lane == 0) { f.vexp = vexp; f.bad_v = bad; }
