@@ -65,6 +65,8 @@ def check(lens, cache, table, q, y, scale, window=0, f32=False, rows=None):
                     ends = 2.0 ** (-36.5 if f32 else -28.5) * np.abs(w).max() * np.abs(c).sum(0)
                     tol = 2 * weight * mean + ends + (2.0 ** -126 if y.dtype is torch.float32 else HALF16 * np.abs(ref) + 2.0 ** -25)
                     worst = np.abs(out - ref) / tol
+                    if y.dtype is torch.float16:     # from 65520 on, half a step above its largest number, fp16 rounds to infinity
+                        worst = np.where(np.abs(ref) + tol < 65520, worst, np.where(np.isinf(out), out * ref < 0, (np.abs(ref) - tol >= 65520) + worst))
                     assert (worst <= 1).all(), (b, i, g, float(np.nanmax(worst)), out[:4], ref[:4])
         row += a
     assert (got[row:] == 0.5).all()
@@ -179,3 +181,74 @@ def test_steps_without_blocks(f32, small, dim, new):
     run(lens, cache, table, start, kv_len, q, y, 0.05)
     check(lens, cache, table, q, y, 0.05, f32=f32)
     assert K.device_error() == 7
+
+
+@pytest.mark.parametrize("huge", [2.0 ** 40, 1e20, 3e38])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("dim,new", [(64, 1), (64, 9), (64, 40), (128, 5), (128, 40), (256, 3)])
+def test_huge_scales_in_front_of_the_window(huge, f32, dim, new):
+    """Blocks that slid out of the window are in the table still."""
+    lens, window = [(300, new), (140, new)], 60
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(dim), lens, 2, 4, 16, dim, torch.float32 if f32 else torch.float16)
+    for b, (n, _) in enumerate(lens):
+        gone = table[b, :(n - new - window + 1) // 16].long()
+        cache.tensors[2][gone] = huge
+        cache.tensors[3][gone] = -huge
+    run(lens, cache, table, start, kv_len, q, y, 0.05, window)
+    check(lens, cache, table, q, y, 0.05, window, f32=f32)
+    no_error()
+
+
+@pytest.mark.parametrize("huge", [2.0 ** 24, 1e20, 2e36])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("dim,new", [(64, 20), (64, 5), (64, 70), (128, 18), (128, 70), (256, 18)])
+@pytest.mark.parametrize("window", [0, 30])
+def test_huge_scales_that_only_some_rows_see(huge, f32, dim, new, window):
+    """The last block's values are far above all others: the rows in front of it do not see them, and with a window the last rows do not see
+    a block in front that the first ones do."""
+    n = 96 + new
+    lens = [(n, new)]
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(dim), lens, 2, 4, 16, dim, torch.float32)
+    if not f32:
+        q, y = q.half(), y.half()
+    cache.tensors[3][table[0, (n - 1) // 16].long()] *= huge
+    if window:
+        cache.tensors[3][table[0, (n - new - 3) // 16].long()] *= huge
+    y = y.float()                                # the large ones leave fp16's range
+    run(lens, cache, table, start, kv_len, q, y, 0.05, window)
+    check(lens, cache, table, q, y, 0.05, window, f32=True)
+    no_error()
+
+
+@pytest.mark.parametrize("dim,new", [(64, 18), (64, 70), (128, 18), (128, 70), (256, 18)])
+def test_fp16_rows_that_do_not_see_the_large_scales(dim, new):
+    n = 96 + new
+    lens = [(n, new)]
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(dim), lens, 2, 4, 16, dim, torch.float16)
+    cache.tensors[3].mul_(2.0 ** -6)
+    last = (n - 1) // 16
+    cache.tensors[3][table[0, last].long()] *= 2.0 ** 12
+    run(lens, cache, table, start, kv_len, q, y, 0.05)
+    check(lens, cache, table, q, y, 0.05)
+    no_error()
+
+
+@pytest.mark.parametrize("power,apart", [(36, (44, 20, -40)), (12, (44, 20, -40)), (12, (80, 60, -75)), (12, (-60, 10, -60))])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("dim,new", [(64, 1), (64, 20), (128, 5), (128, 70), (256, 2)])
+def test_a_huge_scale_under_a_vanishing_weight(power, apart, f32, dim, new):
+    """One block's keys point away from the queries, so its weights vanish beside the others', and its V scale makes up for a part of that."""
+    lens = [(200, new)]
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(dim), lens, 2, 4, 16, dim, torch.float32 if f32 else torch.float16)
+    q.copy_(q.abs() + 0.25)
+    cache.tensors[3].mul_(2.0 ** power)
+    for j, more, sign in zip((4, 9, 10), apart, (-1, -1, 1)):
+        block = int(table[0, j])
+        cache.tensors[0][block].clamp_(20, 127)
+        cache.tensors[0][block].mul_(sign)
+        cache.tensors[2][block] = 2.0 ** -6
+        cache.tensors[3][block] *= 2.0 ** more
+    scale = 60 / (dim * 1.5 * 2.0 ** -6 * 70)    # scores of the blocks around -60 and 60
+    run(lens, cache, table, start, kv_len, q, y, scale)
+    check(lens, cache, table, q, y, scale, f32=f32)
+    no_error()

@@ -20,14 +20,16 @@
 // pairs two tokens' codes by byte permutes.  P^T is the transposed accumulator of S^T (movmatrix).  tau = 0 5 2 7 4 1 6 3:
 // with the copies' 128-byte swizzle both reads are free of bank conflicts (even and odd g differ in bit 2 of the row, even
 // rows of the c's are all different).  A code becomes fp16 exactly: 0x6400 | (code + 128) is 1152 + code.
-//   Online softmax per warp: the running maximum m moves only when some score exceeds it by more than a slack of 8 in the
-// exponent (one vote per 16 tokens instead of a reduction); p = 2^(s - m + 4) then stays inside fp16 and ends at 2^-28 of the
-// largest weight.  Scores, maxima, sums and accumulators are fp32; p is rounded to
+//   Online softmax per warp and row, whose reference c is the largest exponent (rounded to an integer) not of a weight but of a weight
+// TIMES its V scale: p = 2^(s - c + 4) sv then stays inside fp16 and ends at 2^-29 of the row's largest such product, whatever the
+// scales of blocks are that the row does not see or hardly weighs.  c moves only when exceeded by more than a slack of 8 (one
+// vote per 16 tokens instead of a reduction).  The weights' sum, relative to 2^c too, is up to 2^127 apart from 1, which fp32
+// holds.  Scores, references, sums and accumulators are fp32; p is rounded to
 // fp16 for the second product (relative 2^-11, against fp16 outputs with the same step).  With fp32 inputs or outputs
 // (SPLIT) q and p go in as two fp16 terms each, 22 bits; a row of fp32 queries is first brought near the upper end of fp16's
 // range by a power of two, which its scores are divided by.
 //   A tile of 16 tokens lies in one block (block sizes are multiples of 16), so its scales are two scalars: sk goes into
-// the score's factor, sv over a running power of two into p.
+// the score's factor, sv into p.
 //
 // Measured: 64 sequences of 3000 to 12000 tokens, 64 / 8 heads of 128 (958 MB) 193 us = 4.96 TB/s, 160 with the arithmetic
 // left out; one sequence of 8192 tokens 18 us with the join, of which the copies and the arithmetic take 4.
@@ -46,13 +48,15 @@ constexpr int kAttnMaxSeqs = 4096;
 constexpr int kAttnStep = 128;                      // tokens of a step: eight tiles of 16, dealt to the warps in turn
 constexpr int kAttnMinSteps = 1;                    // steps a CTA gets at least
 constexpr uint32_t kAttnHidden = 0xfffe5afeu;       // in place of a K scale: 16 tokens without a block (a NaN no arithmetic makes)
-// A score may exceed the running maximum by `slack` before that moves, a block's V scale the running power of two by
-// kAttnScaleSlack, and a scale is below twice its power of two: p = 2^(s - m + lift) sv / 2^vrun < 2^(slack + lift + 3), which
-// has to stay below 2^16.  With two terms per weight (SPLIT) every bit that the slack does not take goes to small weights.
-__host__ __device__ constexpr float attn_slack(bool split) { return split ? 0.f : 8.f; }
+// The exponent of a weight's product with its V scale may exceed c by `slack`, and a scale is below twice its power of two:
+// p = 2^(s - c + lift) sv < 2^(slack + lift + 1), which has to stay below 2^16.  With two terms per weight (SPLIT) more bits go to small
+// weights.
+__host__ __device__ constexpr float attn_slack(bool split) { return split ? 2.f : 8.f; }
 __host__ __device__ constexpr float attn_lift(bool split) { return split ? 12.f : 4.f; }
-constexpr int kAttnScaleSlack = 2;
-static_assert(attn_slack(false) + attn_lift(false) + kAttnScaleSlack + 1 < 16 && attn_slack(true) + attn_lift(true) + kAttnScaleSlack + 1 < 16, "p stays below 2^15");
+static_assert(attn_slack(false) + attn_lift(false) + 1 < 16 && attn_slack(true) + attn_lift(true) + 1 < 16, "p stays in fp16");
+// V scales below 2^kAttnLeast count as that: sums of weights stay below 2^(slack + lift - kAttnLeast) times their number, and products
+// below 2^(kAttnLeast - 29) may vanish.
+constexpr int kAttnLeast = -90;
 
 struct AttnParams {
     const void* q;
@@ -127,6 +131,27 @@ __device__ __forceinline__ uint32_t unbias(uint32_t x) {
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The exponent of a finite V scale
+__device__ __forceinline__ float attn_exponent(float sv) { return (float)max((int)(__float_as_uint(fabsf(sv)) >> 23) - 127, kAttnLeast); }
+// What exponents are moved by for a reference
+__device__ __forceinline__ float attn_shift(bool split, float c) { return c == -INFINITY ? 0.f : attn_lift(split) - c; }
+// The factor 2^(from - to), from <= to, between two references (integers, so it is exact) in two parts: sums of weights may be more than
+// fp32's 2^126 apart and matter still, products do not.
+struct AttnStep {
+    float a, b;
+    __device__ __forceinline__ AttnStep(float from, float to) {
+        const float d = from - to;                          // 2^-252 also where `from`, or both, are -inf
+        a = ex2(fmaxf(d, -126.f));
+        b = ex2(fminf(fmaxf(d + 126.f, -126.f), 0.f));
+    }
+    __device__ __forceinline__ float sum(float x) const { return x * a * b; }
+    __device__ __forceinline__ float products() const { return a * b; }
+};
 // The power of two that brings a row whose largest element is `top` to [2^14, 2^15), where two fp16 terms hold 22 bits of every element
 // down to 2^-17 of the largest, and the others to 2^-39 of that (a row below 2^-112 stays below, and its subnormal numbers are exact).
 __device__ __forceinline__ float attn_up(float top) { return __uint_as_float(min(127 + 14 + 127 - (__float_as_uint(top) >> 23), 253u) << 23); }
@@ -135,11 +160,6 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
     asm volatile(
@@ -430,7 +450,7 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
         }
 
         float acc[NT][KS][4];                                   // [dims 2 mt (+1) of the lane's][rows 2c, 2c + 1]
-        float m[NT][2], l[NT][2];
+        float m[NT][2], l[NT][2];                               // the references c and the sums of the weights
         int last[NT][2], z_min = 0x7fffffff, z_max = -1;        // last key that each of the lane's rows sees (its first is that less the window)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -447,7 +467,6 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
         }
         z_min = __reduce_min_sync(0xffffffffu, z_min);
         z_max = __reduce_max_sync(0xffffffffu, z_max);
-        int vrun = -1000;
 
         // The CTA's tiles are dealt to the warps in turn, eight per step: `mine` is this warp's tile of the step, if below 8.
         // A warp without one waits and arrives all the same: a barrier's parity says which phase it is in only to those
@@ -494,9 +513,11 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
                     }
                 }
             }
-            // ---- masks and the running maximum
+            // ---- masks and the reference
             const float f = f2.x * p.scale_log2;
             const bool whole_tile = !hidden && tok + 15 <= z_min && (p.window <= 0 || tok > z_max - p.window);
+            const bool fine = fabsf(f2.y) <= 3.402823466e38f;
+            const float sv_exp = fine ? attn_exponent(f2.y) : (float)kAttnLeast;
             bool grows = false;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -508,7 +529,7 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
                         const bool seen = !hidden && key <= z && (p.window <= 0 || key > z - p.window);
                         sc[t][i] = seen ? sc[t][i] : -INFINITY;
                     }
-                    grows |= sc[t][i] > m[t][i & 1] + attn_slack(SPLIT);
+                    grows |= sc[t][i] > m[t][i & 1] + (attn_slack(SPLIT) - sv_exp);
                 }
             if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
@@ -518,31 +539,20 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
                         float top = fmaxf(sc[t][i], sc[t][i + 2]);
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        if (top > m[t][i]) {
-                            const float fix = m[t][i] == -INFINITY ? 0.f : ex2(m[t][i] - top);
-                            l[t][i] *= fix;
+                        top = rintf(top + sv_exp);
+                        if (m[t][i] == -INFINITY) m[t][i] = top;        // nothing summed yet
+                        else if (top > m[t][i]) {
+                            const AttnStep by(m[t][i], top);
+                            const float fix = by.products();
+                            l[t][i] = by.sum(l[t][i]);
 #pragma unroll
                             for (int j = 0; j < KS; ++j) { acc[t][j][i] *= fix; acc[t][j][i + 2] *= fix; }
                             m[t][i] = top;
                         }
                     }
             }
-            // ---- the V scale over the running power of two
-            float r = 0.f;
-            if (fabsf(f2.y) <= 3.402823466e38f) {
-                const int e = min(max((int)(__float_as_uint(fabsf(f2.y)) >> 23) - 127, -120), 120);
-                if (e > vrun + kAttnScaleSlack) {
-                    const float fix = vrun > -1000 ? ex2((float)max(vrun - e, -126)) : 0.f;
-                    vrun = e;
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int j = 0; j < KS; ++j)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[t][j][i] *= fix;
-                }
-                r = f2.y * __uint_as_float((uint32_t)(127 - vrun) << 23);
-            } else {                                            // NaN for the rows that see the tile, not for the masked ones
+            const float sv_fine = fine ? f2.y : 0.f;
+            if (!fine) {                                        // NaN for the rows that see the tile, not for the masked ones
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -556,13 +566,13 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
             uint32_t ph[NT][2], pl[SPLIT ? NT : 1][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const float shift0 = attn_lift(SPLIT) - (m[t][0] == -INFINITY ? 0.f : m[t][0]), shift1 = attn_lift(SPLIT) - (m[t][1] == -INFINITY ? 0.f : m[t][1]);
+                const float shift0 = attn_shift(SPLIT, m[t][0]), shift1 = attn_shift(SPLIT, m[t][1]);
                 float e[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     e[i] = ex2(sc[t][i] + (i & 1 ? shift1 : shift0));
                     l[t][i & 1] += e[i];
-                    e[i] *= r;
+                    e[i] *= sv_fine;
                 }
                 const uint32_t h0 = pack_half2(e[0], e[1]), h1 = pack_half2(e[2], e[3]);
                 ph[t][0] = transpose8x8(h0);
@@ -611,18 +621,12 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
         }
 
         // ---- the warps' parts meet, the upper half's with the lower's until one is left, in a fixed order
-        {
-            const float vref = vrun > -1000 ? ex2((float)vrun) : 0.f;
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], o);
-#pragma unroll
-                    for (int j = 0; j < KS; ++j) { acc[t][j][i] *= vref; acc[t][j][i + 2] *= vref; }
-                }
-        }
+                for (int o = 4; o < 32; o <<= 1) l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], o);
 #pragma unroll
         for (int left = kAttnWarps; left > 1; left = (left + 1) / 2) {
             const int half = (left + 1) / 2;
@@ -644,11 +648,13 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
                     float f0[2], f1[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float mo = i ? o.y : o.x, lo = i ? o.w : o.z, top = fmaxf(m[t][i], mo);
-                        f0[i] = m[t][i] == -INFINITY ? 0.f : ex2(m[t][i] - top);
-                        f1[i] = mo == -INFINITY ? 0.f : ex2(mo - top);
-                        l[t][i] = f0[i] * l[t][i] + f1[i] * lo;
-                        m[t][i] = top;
+                        const float mo = i ? o.y : o.x, lo = i ? o.w : o.z;
+                        const bool up = m[t][i] >= mo;                // whose reference stays
+                        const AttnStep by(fminf(m[t][i], mo), fmaxf(m[t][i], mo));
+                        f0[i] = up ? 1.f : by.products();
+                        f1[i] = up ? by.products() : 1.f;
+                        l[t][i] = up ? l[t][i] + by.sum(lo) : by.sum(l[t][i]) + lo;
+                        m[t][i] = fmaxf(m[t][i], mo);
                     }
 #pragma unroll
                     for (int j = 0; j < KS; ++j) {
@@ -732,11 +738,13 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnParam
             float x[V];
 #pragma unroll
             for (int k = 0; k < V; ++k) x[k] = row[32 * k + lane];
-            const float up = fmaxf(top, ml.x), old = top == -INFINITY ? 0.f : ex2(top - up), fix = ml.x == -INFINITY ? 0.f : ex2(ml.x - up);
-            sum = old * sum + fix * ml.y;
+            const bool up = top >= ml.x;                        // whose reference stays
+            const AttnStep by(fminf(top, ml.x), fmaxf(top, ml.x));
+            const float old = up ? 1.f : by.products(), fix = up ? by.products() : 1.f;
+            sum = up ? sum + by.sum(ml.y) : by.sum(sum) + ml.y;
 #pragma unroll
             for (int k = 0; k < V; ++k) v[k] = old * v[k] + fix * x[k];
-            top = up;
+            top = fmaxf(top, ml.x);
         }
     }
     if (share > 1) {
@@ -752,8 +760,9 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnParam
         for (int u = 0; u < WARPS; ++u) top = fmaxf(top, red[u][D]);
 #pragma unroll
         for (int u = 0; u < WARPS; ++u) {
-            const float fix = red[u][D] == -INFINITY ? 0.f : ex2(red[u][D] - top);
-            sum += fix * red[u][D + 1];
+            const AttnStep by(red[u][D], top);
+            const float fix = by.products();
+            sum += by.sum(red[u][D + 1]);
 #pragma unroll
             for (int k = 0; k < V; ++k) v[k] += fix * red[u][32 * k + lane];
         }

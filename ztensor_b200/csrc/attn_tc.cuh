@@ -3,16 +3,16 @@
 // An item is (sequence, 256 rows, kv head) and one CTA; its rows are two tiles of 128 (M of the products).  Per step of 128
 // keys:
 //   S_t = Q_t K^T   (fp16 x fp16 -> fp32 in TMEM, 128 columns)            Q_t, K from shared memory
-//   P_t = 2^(S_t f - m + lift) as fp16, over the columns of S_t
+//   P_t = 2^(S_t f - c + lift) sv as fp16, over the columns of S_t
 //   O_t += P_t V    (P_t from TMEM, V^T from shared memory; D columns)
 // The codes become fp16 operands (exactly) on the way into shared memory, once per step for both tiles: a step's 64 KB of
 // operands cost what a quarter of the exponentials costs.  The scales stay out of the operands: sixteen keys are a chunk of
-// scores in the softmax, whose exponent's factor takes sk and whose weights take sv over a running power of two.
+// scores in the softmax, whose exponent's factor takes sk and whose weights take sv.
 //
 // Roles of the warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread is a row: TMEM lane), then kTcaConv for K codes ->
 // operand and kTcaConv for V (loaded one step ahead, their blocks and scales two), the last issues the products.  The two
-// tiles alternate: while one is in its softmax the tensor cores work for the other.  The running maximum moves only when a score exceeds it by more than a slack
-// (then the row's O is rescaled in TMEM), as does the reference of the V scales.
+// tiles alternate: while one is in its softmax the tensor cores work for the other.  The reference c of a row
+// (attn_q8.cuh) moves only when exceeded by more than a slack; then the row's O is rescaled in TMEM.
 // Operands stand in the canonical K-major layout without swizzle: core matrices of 8 rows x 16 bytes, 128 bytes apart along
 // the contraction; both store patterns below are free of bank conflicts.
 //
@@ -43,8 +43,7 @@ constexpr int kTcaMma = 8 + 2 * kTcaConv;
 constexpr int kTcaThreads = 32 * (kTcaMma + 1);
 
 struct __align__(16) TcaInfo {                  // one step's factors, by groups of 16 keys
-    float ks[8], vs[8];                         // |K scale|; V scale / 2^vexp, 0 where it is not finite
-    int vexp;
+    float ks[8], vs[8], ve[8];                  // |K scale|; V scale, 0 where it is not finite; its exponent
     uint32_t hidden, bad_v;                     // groups without a block; groups whose V scale is not finite
 };
 
@@ -54,10 +53,10 @@ struct TcaShared {
     uint32_t tmem;
     float down[128];                            // fp32 queries: what a row's scores are multiplied by
 };
-static_assert(sizeof(TcaShared) <= 1024, "the end of tca_smem");
+static_assert(sizeof(TcaShared) <= 2048, "the end of tca_smem");
 template <int D>
 __host__ __device__ constexpr int tca_smem() {
-    const int n = 256 * D * 2 + 4 * kTcaKeys * D * 2 + 1024;
+    const int n = 256 * D * 2 + 4 * kTcaKeys * D * 2 + 2048;
     return n < 120 * 1024 ? 120 * 1024 : n;     // one CTA per SM: it holds all of TMEM
 }
 
@@ -328,13 +327,9 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.info_full[i & 3]);
             } else if (warp == 8 + kTcaConv) {
-                uint32_t top = fine ? __float_as_uint(fabsf(sc)) >> 23 : 0u;
-#pragma unroll
-                for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const int vexp = min(max((int)top - 127, -120), 120);       // -120 without any: the reference stays where real scales put it
                 const uint32_t bad = __ballot_sync(0xffffffffu, blk >= 0 && !fine) & 255u;
-                if (lane < 8) f.vs[lane] = fine ? sc * __uint_as_float((uint32_t)(127 - vexp) << 23) : 0.f;
-                if (lane == 0) { f.vexp = vexp; f.bad_v = bad; }
+                if (lane < 8) { f.vs[lane] = fine ? sc : 0.f; f.ve[lane] = fine ? attn_exponent(sc) : (float)kAttnLeast; }
+                if (lane == 0) f.bad_v = bad;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.info_full[i & 3]);
             }
@@ -440,8 +435,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
         const int z = live ? min(base + r / p.group, it.s.len - 1) : -1;    // last key the row sees
         const int z_lo = p.window > 0 ? z - p.window : -1;                  // the last one in front of those it sees
         const float scale = fabsf(p.scale_log2), down = SPLIT ? sh.down[r - it.r0] : 1.f;
-        float m = -INFINITY, l = 0.f;
-        int vrun = -1000;
+        float m = -INFINITY, l = 0.f, shift = 0.f;              // the reference c, the sum of the weights, what exponents are moved by
         for (int i = 0; i < n; ++i) {
             if (!wait(&sh.info_full[i & 3], i >> 2) || !wait(&sh.s_full[t], i)) break;
             tc_fence_after();
@@ -485,17 +479,14 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
             for (int c = 0; c < 8; ++c) {
                 fk[c] = info.ks[c] * scale;
                 if constexpr (SPLIT) fk[c] *= down;
-                top = tops[c] != -INFINITY ? fmaxf(top, tops[c] * fk[c]) : top;         // -inf may meet a factor of 0
+                top = tops[c] != -INFINITY ? fmaxf(top, tops[c] * fk[c] + info.ve[c]) : top;        // -inf may meet a factor of 0
             }
-            const bool grows = top > m + attn_slack(SPLIT), scale_grows = info.vexp > vrun + kAttnScaleSlack;
-            if (__any_sync(0xffffffffu, grows) || scale_grows) {
-                const float m_new = fmaxf(m, top);
-                float fix = m == -INFINITY ? 0.f : ex2(m - m_new);
-                l *= fix;
-                if (scale_grows) {
-                    fix *= vrun > -1000 ? ex2((float)max(vrun - info.vexp, -126)) : 0.f;
-                    vrun = info.vexp;
-                }
+            if (__any_sync(0xffffffffu, top > m + attn_slack(SPLIT))) {
+                const float m_new = fmaxf(m, rintf(top));
+                const AttnStep by(m, m_new);
+                const float fix = by.products();
+                l = by.sum(l);
+                shift = attn_shift(SPLIT, m_new);
                 if (i > 0) {
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
@@ -512,7 +503,6 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                 }
                 m = m_new;
             }
-            const float m_safe = m == -INFINITY ? 0.f : m, shift = attn_lift(SPLIT) + (float)max(info.vexp - vrun, -100) - m_safe;
             f2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};
             float fv[8];
 #pragma unroll
@@ -541,7 +531,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
             };
             if (edge) weights(std::true_type());
             else weights(std::false_type());
-            l = fmaf((sums[0].x + sums[0].y) + (sums[1].x + sums[1].y), ex2((float)-max(info.vexp - vrun, -100)), l);
+            l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
             if (info.bad_v)
                 for (int g = 0; g < 8; ++g)                     // a V scale that is not finite: NaN for the rows that see its keys
                     if (info.bad_v >> g & 1 && max(16 * g, a + 1) <= min(16 * g + 15, b)) l = __int_as_float(0x7fc00000);
@@ -551,8 +541,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
         }
         if (n > 0 && wait(&sh.o_full[t], 0)) tc_fence_after();
         // ---- the row's output, or its part
-        const float vref = n > 0 && vrun > -1000 ? ex2((float)vrun) : 0.f;
-        const float inv = l > 0.f || l != l ? vref / l : 0.f;
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
         float* part = tp.parts + (((long long)blockIdx.x * tp.splits + blockIdx.y) * tca_rows(SPLIT) + (r - it.r0)) * (D + 2);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
@@ -565,7 +554,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
             if (!live || !ok) continue;
             if (tp.splits > 1) {
 #pragma unroll
-                for (int k = 0; k < 32; k += 2) *reinterpret_cast<float2*>(part + 32 * c + k) = make_float2(o[k] * vref, o[k + 1] * vref);
+                for (int k = 0; k < 32; k += 2) *reinterpret_cast<float2*>(part + 32 * c + k) = make_float2(o[k], o[k + 1]);
             } else {
 #pragma unroll
                 for (int k = 0; k < 32; k += 8) {
@@ -605,8 +594,9 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const TcaParams tp) {
     float sum = 0.f, v[D / 32] = {};
     for (int u = 0; u < tp.splits; ++u) {
         const float* row = row_of(u);
-        const float fix = row[D] == -INFINITY ? 0.f : exp2f(row[D] - top);
-        sum += fix * row[D + 1];
+        const AttnStep by(row[D], top);
+        const float fix = by.products();
+        sum += by.sum(row[D + 1]);
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) v[k] += fix * row[32 * k + lane];
     }
