@@ -384,7 +384,7 @@ cudaError_t ztq_kv_read_q8(const ZtqKvCache* cache, const int* slots, int tokens
  * workspace: >= ztq_attn_q8_workspace_bytes(...) of the same sizes, 16-byte aligned, overwritten; calls that share one must not overlap on the GPU
  * (two captured graphs that may run at once need one each).  sequences <= 4096.
  * With ZTQ_X_F32 or ZTQ_Y_F32 queries (of any size) and weights enter the products with 22 bits, else weights with 11; scores,
- * softmax sums and outputs are summed in fp32.  A weight times its V scale keeps these bits down to 2^-23 (else 2^-18) of the row's
+ * softmax sums and outputs are summed in fp32.  A weight times its V scale keeps these bits down to 2^-15 (else 2^-18) of the row's
  * largest such product and is held to 2^-36 (2^-28) of it; V scales below 2^-90 count as that.  Flags: ZTQ_X_F32, ZTQ_Y_F32, ZTQ_NO_PDL. */
 size_t ztq_attn_q8_workspace_bytes(int tokens, int sequences, int max_new, int q_heads, int kv_heads, int head_dim);
 cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_head, long long y_token, long long y_head, int tokens, int q_heads,

@@ -73,7 +73,7 @@ struct AttnParams {
     float* parts;                                   // [grid][2] slots of 8 NT (D + 2) floats
     int seqs, tokens, max_new, q_heads, kv_heads, group, width, shift, blocks, window;
     float scale_log2;                               // softmax scale times log2(e)
-    int x_f32, y_f32, vec, y_wide;                  // vec, y_wide: 8-byte reads of q, 16-byte stores of y
+    int x_f32, y_f32, vec, y_wide;                  // vec, y_wide: reads of four elements of q, 16-byte stores of y
     int min_rows, max_rows;                         // sequences with more or fewer rows per kv head belong to another kernel
 };
 

@@ -198,12 +198,22 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
             const int row = it.r0 + r;
             float x[CG / 4][8], top = 0.f;
 #pragma unroll
-            for (int j = 0; j < CG / 4; ++j)
+            for (int j = 0; j < CG / 4; ++j) {
+                const float* src = static_cast<const float*>(p.q) + query_at(row) + 8 * (4 * j + (lane >> 3));
+                if (row >= it.r1) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    x[j][k] = row < it.r1 ? static_cast<const float*>(p.q)[query_at(row) + 8 * (4 * j + (lane >> 3)) + k] : 0.f;
-                    top = fmaxf(top, fabsf(x[j][k]));
+                    for (int k = 0; k < 8; ++k) x[j][k] = 0.f;
+                } else if (p.vec) {
+                    const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+                    x[j][0] = a.x; x[j][1] = a.y; x[j][2] = a.z; x[j][3] = a.w;
+                    x[j][4] = b.x; x[j][5] = b.y; x[j][6] = b.z; x[j][7] = b.w;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[j][k] = src[k];
                 }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[j][k]));
+            }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             float up = attn_up(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)));
             if (lane < 8) sh.down[r] = attn_down(up);

@@ -164,7 +164,7 @@ cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_h
     p.scale_log2 = scale * 1.44269504088896340736f;
     p.x_f32 = (flags & ZTQ_X_F32) ? 1 : 0;
     p.y_f32 = (flags & ZTQ_Y_F32) ? 1 : 0;
-    p.vec = ((uintptr_t)q & 7) == 0 && q_token % 4 == 0 && q_head % 4 == 0;
+    p.vec = ((uintptr_t)q & (p.x_f32 ? 15 : 7)) == 0 && q_token % 4 == 0 && q_head % 4 == 0;
     const int wide = p.y_f32 ? 4 : 8;
     p.y_wide = ((uintptr_t)y & 15) == 0 && y_token % wide == 0 && y_head % wide == 0;
     p.min_rows = 1;
