@@ -380,7 +380,8 @@ cudaError_t ztq_kv_read_q8(const ZtqKvCache* cache, const int* slots, int tokens
  * of kv_heads; head h reads kv head h / (q_heads / kv_heads).  Rows of sequence b: query_start[b] .. query_start[b + 1];
  * rows behind the last sequence are left as they were; a row that sees nothing becomes 0.  scale_bits: the softmax
  * scale's float32 bits.  max_new: most rows of one sequence (a sequence with more is left out and sets the device error
- * word to 8).  A block table entry outside the cache hides its tokens and sets the error word to 7.
+ * word to 8).  A block table entry outside the cache hides its tokens and sets the error word to 7; entries in front of the
+ * window of a sequence's first row are not looked at.
  * workspace: >= ztq_attn_q8_workspace_bytes(...) of the same sizes, 16-byte aligned, overwritten; calls that share one must not overlap on the GPU
  * (two captured graphs that may run at once need one each).  sequences <= 4096.
  * With ZTQ_X_F32 or ZTQ_Y_F32 queries (of any size) and weights enter the products with 22 bits, else weights with 11; scores,

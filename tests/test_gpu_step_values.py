@@ -252,3 +252,19 @@ def test_a_huge_scale_under_a_vanishing_weight(power, apart, f32, dim, new):
     run(lens, cache, table, start, kv_len, q, y, scale)
     check(lens, cache, table, q, y, scale, f32=f32)
     no_error()
+
+
+# ------------------------------------------------------------------ what a window has left behind
+
+@pytest.mark.parametrize("dim,size", [(64, 16), (128, 64), (256, 32), (64, 128)])
+@pytest.mark.parametrize("new", [1, 5, 40, 90])
+@pytest.mark.parametrize("window", [1, 17, 100])
+def test_blocks_in_front_of_the_window_may_be_gone(dim, size, new, window):
+    """A server gives back the blocks in front of the window and marks them -1: nobody sees them, so there is no error."""
+    lens = [(700, new), (90 + new, new), (1, 1)]
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(dim), lens, 2, 4, size, dim, torch.float16)
+    for b, (n, a) in enumerate(lens):
+        table[b, :max(0, n - a - window + 1) // size] = -1
+    run(lens, cache, table, start, kv_len, q, y, 0.1, window)
+    check(lens, cache, table, q, y, 0.1, window)
+    no_error()

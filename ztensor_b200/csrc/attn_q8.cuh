@@ -103,6 +103,8 @@ __device__ __forceinline__ void attn_span(const AttnParams& p, const AttnSeq& s,
     hi = min(max(z + 1, 0), s.len);
     lo = p.window > 0 ? (int)min(max((long long)a - p.window + 1, 0ll), (long long)hi) : 0;
 }
+// Whether the block that holds token `tok` holds any of the keys [lo, hi): what lies in front of a window may have lost its block.
+__device__ __forceinline__ bool attn_in_span(int tok, int lo, int hi, int shift) { return tok < hi && tok >> shift >= lo >> shift; }
 __device__ __forceinline__ int attn_steps(int lo, int hi, int step) {
     return max(1, (hi + step - 1) / step - lo / step);          // an item without keys still writes its zeros
 }
@@ -338,7 +340,7 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
             auto look = [&](int first) {                        // the block of this lane's group, -1 where there is none
                 const int step = first + (lane >> 3), tok = (it.lo / kAttnStep + step) * kAttnStep + 16 * (lane & 7);
                 int blk = -1;
-                if (step < step1 && tok < it.hi) {
+                if (step < step1 && attn_in_span(tok, it.lo, it.hi, p.shift)) {
                     blk = table[tok >> p.shift];
                     if ((unsigned)blk >= (unsigned)p.blocks) {
                         report_error(ZTQ_ERR_BLOCK);

@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
         auto look = [&](int kt) {
             const int tok = kt * kTcaKeys + 16 * (lane & 7);
             int blk = -1;
-            if (kt < kt1 && tok < it.hi) {
+            if (kt < kt1 && attn_in_span(tok, it.lo, it.hi, p.shift)) {
                 blk = table[tok >> p.shift];
                 if ((unsigned)blk >= (unsigned)p.blocks) {
                     report_error(ZTQ_ERR_BLOCK);
