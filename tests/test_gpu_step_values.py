@@ -268,3 +268,40 @@ def test_blocks_in_front_of_the_window_may_be_gone(dim, size, new, window):
     run(lens, cache, table, start, kv_len, q, y, 0.1, window)
     check(lens, cache, table, q, y, 0.1, window)
     no_error()
+
+
+# ------------------------------------------------------------------ behind one another
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_prompt_attention_between_tensor_core_products(captured):
+    """Kernels that hold all of an SM's tensor memory, started in one another's shadow: attention over a prompt between products."""
+    from oracle import oracle as O
+    from tests import gpu_util as G
+    lens, n, k = [(600, 300)], 512, 1024
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(3), lens, 8, 4, 64, 128, torch.float16)
+    rng = U.seeded(4)
+    qd, meta = G.upload_w4g(O.quantize_gptq(U.make_weights(rng, n, k), 128))
+    x, out = torch.randn(32, k, device=DEV).half(), torch.zeros(32, n, device=DEV)
+    ws, want = torch.empty(K.gemm_w4g_tc_workspace_bytes(n, k, 32), dtype=torch.uint8, device=DEV), torch.zeros(32, n, device=DEV)
+    work = torch.empty(K.attn_q8_workspace_bytes(q.shape[0], 1, 300, 32, 8, 128), dtype=torch.uint8, device=DEV)
+    K.gemm_w4g_tc(qd, meta, x, want, n, k, 128, 32, ws, K.Y_F32)
+    K.attn_q8(q, y, start, kv_len, table, cache, work, 300, 0.1)
+    first = y.clone()
+    check(lens, cache, table, q, y, 0.1, rows=range(0, 300, 41))
+
+    def step():
+        for _ in range(3):
+            K.gemm_w4g_tc(qd, meta, x, out, n, k, 128, 32, ws, K.Y_F32)
+            K.attn_q8(q, y, start, kv_len, table, cache, work, 300, 0.1)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    if captured:
+        with torch.cuda.graph(graph):
+            step()
+    for _ in range(20):
+        y.fill_(0.5), out.zero_()
+        graph.replay() if captured else step()
+    torch.cuda.synchronize()
+    assert torch.equal(y, first) and torch.equal(out, want)
+    no_error()

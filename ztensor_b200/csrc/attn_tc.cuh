@@ -163,7 +163,6 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
     const AttnParams& p = tp.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-    grid_dep_launch();
     grid_dep_wait();
     // the scan's scratch lies where the operands will be
     int* upto = reinterpret_cast<int*>(sk);
@@ -188,6 +187,9 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
     if (warp == kTcaMma) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        // only now: a kernel behind this one that takes tensor memory before its own wait would otherwise wait for this one's end while
+        // holding what this CTA has yet to get
+        grid_dep_launch();
     }
     // queries: 16-byte pieces in K-major order, a phase of eight lanes writes eight rows of one column; scores use |scale|
     auto query_at = [&](int row) { return (it.s.first + row / p.group) * p.q_token + (long long)(it.h * p.group + row % p.group) * p.q_head; };
