@@ -305,3 +305,31 @@ def test_prompt_attention_between_tensor_core_products(captured):
     torch.cuda.synchronize()
     assert torch.equal(y, first) and torch.equal(out, want)
     no_error()
+
+
+# ------------------------------------------------------------------ the ends of a sequence
+
+@pytest.mark.parametrize("positions", [50, 64])
+def test_decode_attention_up_to_its_last_position(positions):
+    """A table rounded up to whole blocks takes more positions than were asked for; all that it takes are right."""
+    from ztensor_b200.stack import DecodeAttention, ProjectionStack
+    st = ProjectionStack("llama3-8b", batch=1, layers=1)
+    att = DecodeAttention(st, blocks=5, block_size=16, max_positions=positions)
+    assert att.table.shape[1] == 4
+    rng, held, rope = U.seeded(15), [], host(K.rope_table(64, 128, 500000.0))
+    for step in range(64):
+        st.x["qkv"].copy_(dev(rng.standard_normal((1, 4096))))
+        st.step(attention=att)
+        torch.cuda.synchronize()
+        assert att.status.tolist() == [0] and att.positions.tolist() == [step]
+        z, out = host(st.y["qkv"]).reshape(1, 48, 128), host(st.x["o"]).reshape(32, 128)
+        held.append((R.rope(z[:, 32:40], rope, np.array([step]), False)[0], z[0, 40:]))
+        k, v = (np.stack([r[j] for r in held]) for j in (0, 1))
+        for h in range(0, 32, 5):
+            kk, vv = k[:, h // 4], v[:, h // 4]
+            ref, mean, _, _ = R.attention(z[:, h], kk, vv, step, 128 ** -0.5, 0)
+            # a code is off by at most one step, 2 max / 127: the keys' moves a score, the values' adds itself
+            key_step, val_step = 2 * np.abs(kk).max() / 127, 2 * np.abs(vv).max() / 127
+            tol = (np.exp(2 * 128 ** -0.5 * key_step * np.abs(z[0, h]).sum()) - 1) * 2 * mean + val_step + 4 * HALF16 * mean
+            assert (np.abs(out[h] - ref[0]) <= tol[0]).all(), (step, h)
+    no_error()

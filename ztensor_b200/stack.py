@@ -90,7 +90,9 @@ class DecodeAttention:
     """What a decode loop keeps between steps for the attention of a ProjectionStack: the sequences' lengths and block
     tables, the pool of free blocks, one paged 8-bit cache per layer, the rotary table and the workspace.  Every step each
     of the stack's `batch` sequences brings one token; set `new` to -1 to end a sequence (its blocks go back to the pool,
-    its rows of that step are padding) and to 0 to let it wait."""
+    its rows of that step are padding) and to 0 to let it wait.  `max_positions` counts in whole blocks.  A sequence that the
+    plan refuses (`status`: 1 the pool is short of blocks, 2 its table is full) keeps its length, and its row of `out` becomes zeros:
+    a loop looks at `status` where it reads back the step's result, and gives such a sequence the same token again."""
 
     def __init__(self, stack: "ProjectionStack", blocks: int, block_size: int = 64, max_positions: int = 8192, rope_base: float = 500000.0, **rope_scaling):
         _, _, _, qh, kvh = SHAPES[stack.model]
@@ -102,7 +104,7 @@ class DecodeAttention:
         self.ring_state[1] = blocks
         self.kv_len, self.start, self.positions, self.slots, self.status = i32(b), i32(b + 1), i32(b), i32(b), i32(b)
         self.caches = [K.KvCache.empty(blocks, self.kv_heads, block_size, self.dim, device=dev) for _ in stack.layers]
-        self.rope = K.rope_table(max_positions, self.dim, rope_base, **rope_scaling)
+        self.rope = K.rope_table(self.table.shape[1] * block_size, self.dim, rope_base, **rope_scaling)     # as many positions as the plan admits
         self.workspace = torch.empty(K.attn_q8_workspace_bytes(b, b, 1, self.q_heads, self.kv_heads, self.dim), dtype=torch.uint8, device=dev)
 
     def begin_step(self):
