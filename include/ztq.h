@@ -360,7 +360,7 @@ typedef struct ZtqKvCache {
 } ZtqKvCache;
 
 /* Rotates the queries into q_out (q_heads 0: none; q_out may be q) and appends the step's keys (rotated) and values to the
- * cache at `slots` (negative: the row is skipped).  table NULL: nothing is rotated.  Strides in elements.
+ * cache at `slots` (negative: the row is skipped, and a position outside the table is no error).  table NULL: nothing is rotated.  Strides in elements.
  * The scale of a (block, head) becomes the smallest power of two that holds the new rows' largest value in 127 steps, or
  * stays if it is larger already and the block held rows of the sequence (slot offset > 0); codes in the block are rounded
  * to a grown scale.  A block whose new rows are not finite gets the scale NaN until it is begun anew.

@@ -333,3 +333,30 @@ def test_decode_attention_up_to_its_last_position(positions):
             tol = (np.exp(2 * 128 ** -0.5 * key_step * np.abs(z[0, h]).sum()) - 1) * 2 * mean + val_step + 4 * HALF16 * mean
             assert (np.abs(out[h] - ref[0]) <= tol[0]).all(), (step, h)
     no_error()
+
+
+@pytest.mark.parametrize("x32", [False, True])
+def test_refused_sequences_raise_no_error(x32):
+    """A sequence whose table is full gets status 2 and no slots: its rows' positions lie behind the rotary table, which is no error; a row with a
+    slot there is one."""
+    dtype = torch.float32 if x32 else torch.float16
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    z = lambda n: torch.zeros(n, dtype=torch.int32, device=DEV)  # noqa: E731
+    kv_len, start, pos, slots, status, nxt = z(3), z(4), z(40), z(40), z(3), z(3)
+    table = i(0, 1, 2, 3, -1, -1).view(3, 2)
+    K.kv_plan(i(32, 20, 0), i(1, 5, 34), table, i(4, 5, 0, 1, 2, 3), i(0, 2), z(2), nxt, kv_len, start, pos, slots, status, 16)
+    assert status.tolist() == [2, 0, 2] and pos.tolist()[:7] == [32, 20, 21, 22, 23, 24, 0] and slots.tolist()[:2] == [-1, 52]
+    cache, rope = K.KvCache.empty(6, 1, 16, 64), K.rope_table(32, 64, 10000.0)
+    x = torch.randn(40, 4, 64, device=DEV).to(dtype)
+    q, k, v = x.split([2, 1, 1], 1)
+    out = torch.zeros(40, 2, 64, dtype=dtype, device=DEV)
+    K.rope_append_q8(q, k, v, out, slots, cache, rope, pos)
+    no_error()
+    assert torch.isfinite(out[1:38]).all()
+    y = torch.full_like(out, 0.5)
+    K.attn_q8(out, y, start, kv_len, table, cache, torch.empty(K.attn_q8_workspace_bytes(40, 3, 40, 2, 1, 64), dtype=torch.uint8, device=DEV), 40, 0.125)
+    assert (y[0] == 0).all() and torch.isfinite(y).all() and (y[6:] == 0).all()
+    no_error()
+    slots[0] = 5 * 16
+    K.rope_append_q8(q, k, v, out, slots, cache, rope, pos)
+    assert K.device_error() == 6 and K.device_error() == 0 and torch.isnan(out[0]).all()

@@ -157,17 +157,18 @@ __device__ __forceinline__ void rotate_unit(bool pairs, const float2 (&cs)[8], f
     }
 }
 
-// The table row of a position; NULL (the rotated part becomes NaN) where it lies outside the table.
-__device__ __forceinline__ const float2* rope_row(const RopeParams& r, int pos) {
+// The table row of a position; NULL (the rotated part becomes NaN) where it lies outside the table.  That is an error unless the
+// row has a slot, and a negative one: the plan gives such to a sequence that it refuses, whose positions may go on behind the table.
+__device__ __forceinline__ const float2* rope_row(const RopeParams& r, int pos, const int* slot = nullptr) {
     if (pos < 0 || pos >= r.table_rows) {
-        report_error(ZTQ_ERR_POSITION);
+        if (!slot || *slot >= 0) report_error(ZTQ_ERR_POSITION);
         return nullptr;
     }
     return r.table + (long long)pos * r.half;
 }
 
 template <bool XF32, bool YF32>
-__device__ __forceinline__ void rope_heads(const RopeParams& r, const HeadsIn& x, const HeadsIn& y, int t0, int t1, int h0, int h1, int dim, bool vec) {
+__device__ __forceinline__ void rope_heads(const RopeParams& r, const HeadsIn& x, const HeadsIn& y, int t0, int t1, int h0, int h1, int dim, bool vec, const int* slots = nullptr) {
     const int units = dim >> 4, pairs = kTokenTile * units, strides = kRopeThreads / pairs;      // threads of one head: at most the CTA's
     const int at = threadIdx.x % pairs, j = at % units, t = t0 + at / units, first = threadIdx.x / pairs;
     if (first >= strides || t >= t1) return;
@@ -175,7 +176,7 @@ __device__ __forceinline__ void rope_heads(const RopeParams& r, const HeadsIn& x
     bool rotated;
     unit_offsets(r, j, e0, e1, rotated);
     float2 cs[8];
-    if (rotated) load_turn(rope_row(r, r.positions[t]), j, cs);
+    if (rotated) load_turn(rope_row(r, r.positions[t], slots ? slots + t : nullptr), j, cs);
     const long long src = t * x.token, dst = t * y.token;
 #pragma unroll 4
     for (int h = h0 + first; h < h1; h += strides) {
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const Appe
     const int kv_parts = 2 * p.kv_heads, kv_ctas = (int)gridDim.x - p.q_ctas;
     if ((int)blockIdx.x >= kv_ctas) {
         const int at = blockIdx.x - kv_ctas, t0 = at / p.q_groups * kTokenTile, h0 = at % p.q_groups * p.q_group;
-        rope_heads<XF32, YF32>(p.rope, p.q, p.qo, t0, min(t0 + kTokenTile, p.tokens), h0, min(h0 + p.q_group, p.q_heads), p.dim, p.vec);
+        rope_heads<XF32, YF32>(p.rope, p.q, p.qo, t0, min(t0 + kTokenTile, p.tokens), h0, min(h0 + p.q_group, p.q_heads), p.dim, p.vec, p.slots);
         return;
     }
     const int tile = blockIdx.x / kv_parts, which = blockIdx.x % kv_parts, t0 = tile * p.kv_tile;
