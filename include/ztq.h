@@ -420,7 +420,7 @@ int ztq_check_sm100(void);          /* 1 when the current device is compute capa
  * dependent launch on the device at hand: the part of a small GEMV's time that no kernel change can remove. */
 cudaError_t ztq_probe_launch(int grid, int threads, int smem_bytes, int flags, cudaStream_t stream);
 int ztq_abi_version(void);
-/* Reads and clears the device-side error word (0 = none; see ztq_common.cuh).
+/* Reads and clears the device-side error word (0 = none; see ztq_common.cuh): the first error of one of the operators that had any.
  * Synchronises the device: a diagnostic call, not for the hot path. */
 int ztq_device_error(void);
 

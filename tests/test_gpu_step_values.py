@@ -360,3 +360,15 @@ def test_refused_sequences_raise_no_error(x32):
     slots[0] = 5 * 16
     K.rope_append_q8(q, k, v, out, slots, cache, rope, pos)
     assert K.device_error() == 6 and K.device_error() == 0 and torch.isnan(out[0]).all()
+
+
+def test_device_error_clears_everything():
+    """Errors of several operators before one look at the error word: it names one of them, and nothing is left behind."""
+    rope = K.rope_table(10, 64, 10000.0)
+    x = torch.ones(1, 2, 64, device=DEV)
+    K.rope(x, torch.zeros_like(x), rope, torch.tensor([10], dtype=torch.int32, device=DEV))
+    lens = [(40, 1)]
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(5), lens, 1, 2, 16, 64, torch.float16)
+    table[0, 1] = -5
+    run(lens, cache, table, start, kv_len, q, y, 0.1)
+    assert K.device_error() in (6, 7) and K.device_error() == 0

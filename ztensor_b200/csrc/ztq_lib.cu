@@ -1222,9 +1222,12 @@ int ztq_abi_version(void) { return 1; }
 
 int ztq_device_error(void) {
     if (cudaDeviceSynchronize() != cudaSuccess) return -1;
-    for (auto take : {&take_error, &ztq_take_error_step, &ztq_take_error_attn})   // one word per translation unit
-        if (int e = take()) return e;
-    return 0;
+    int first = 0;
+    for (auto take : {&take_error, &ztq_take_error_step, &ztq_take_error_attn}) {  // one word per translation unit: all are cleared
+        const int e = take();
+        if (first == 0) first = e;
+    }
+    return first;
 }
 
 }  // extern "C"
