@@ -20,10 +20,10 @@
 // pairs two tokens' codes by byte permutes.  P^T is the transposed accumulator of S^T (movmatrix).  tau = 0 5 2 7 4 1 6 3:
 // with the copies' 128-byte swizzle both reads are free of bank conflicts (even and odd g differ in bit 2 of the row, even
 // rows of the c's are all different).  A code becomes fp16 exactly: 0x6400 | (code + 128) is 1152 + code.
-//   Online softmax per warp and row, whose reference c is the largest exponent (rounded to an integer) not of a weight but of a weight
-// TIMES its V scale: p = 2^(s - c + 4) sv then stays inside fp16 and ends at 2^-29 of the row's largest such product, whatever the
+//   Online softmax per warp and row, whose reference c is the largest exponent not of a weight but of a weight TIMES the power of two of
+// its V scale: p = 2^(s - c + 4) sv then stays inside fp16 and ends at 2^-29 of the row's largest such product, whatever the
 // scales of blocks are that the row does not see or hardly weighs.  c moves only when exceeded by more than a slack of 8 (one
-// vote per 16 tokens instead of a reduction).  The weights' sum, relative to 2^c too, is up to 2^127 apart from 1, which fp32
+// vote per 16 tokens instead of a reduction); it is not rounded, so that a weight that outweighs all others is exact.  The weights' sum, relative to 2^c too, is up to 2^127 apart from 1, which fp32
 // holds.  Scores, references, sums and accumulators are fp32; p is rounded to
 // fp16 for the second product (relative 2^-11, against fp16 outputs with the same step).  With fp32 inputs or outputs
 // (SPLIT) q and p go in as two fp16 terms each, 22 bits; a row of fp32 queries is first brought near the upper end of fp16's
@@ -142,8 +142,8 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float attn_exponent(float sv) { return (float)max((int)(__float_as_uint(fabsf(sv)) >> 23) - 127, kAttnLeast); }
 // What exponents are moved by for a reference
 __device__ __forceinline__ float attn_shift(bool split, float c) { return c == -INFINITY ? 0.f : attn_lift(split) - c; }
-// The factor 2^(from - to), from <= to, between two references (integers, so it is exact) in two parts: sums of weights may be more than
-// fp32's 2^126 apart and matter still, products do not.
+// The factor 2^(from - to), from <= to, between two references in two parts: sums of weights may be more than fp32's 2^126 apart and
+// matter still, products do not.  Both take the same factor, so its error of 2^-22 drops out.
 struct AttnStep {
     float a, b;
     __device__ __forceinline__ AttnStep(float from, float to) {
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
                         float top = fmaxf(sc[t][i], sc[t][i + 2]);
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        top = rintf(top + sv_exp);
+                        top += sv_exp;
                         if (m[t][i] == -INFINITY) m[t][i] = top;        // nothing summed yet
                         else if (top > m[t][i]) {
                             const AttnStep by(m[t][i], top);

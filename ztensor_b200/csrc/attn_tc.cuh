@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
                 top = tops[c] != -INFINITY ? fmaxf(top, tops[c] * fk[c] + info.ve[c]) : top;        // -inf may meet a factor of 0
             }
             if (__any_sync(0xffffffffu, top > m + attn_slack(SPLIT))) {
-                const float m_new = fmaxf(m, rintf(top));
+                const float m_new = fmaxf(m, top);
                 const AttnStep by(m, m_new);
                 const float fix = by.products();
                 l = by.sum(l);
