@@ -381,7 +381,7 @@ cudaError_t ztq_kv_read_q8(const ZtqKvCache* cache, const int* slots, int tokens
  * rows behind the last sequence are left as they were; a row that sees nothing becomes 0.  scale_bits: the softmax
  * scale's float32 bits.  max_new: most rows of one sequence (a sequence with more is left out and sets the device error
  * word to 8).  A block table entry outside the cache hides its tokens and sets the error word to 7; entries in front of the
- * window of a sequence's first row are not looked at.
+ * window of a sequence's first row are not looked at.  A scale that is not finite makes the rows that see its tokens NaN.
  * workspace: >= ztq_attn_q8_workspace_bytes(...) of the same sizes, 16-byte aligned, overwritten; calls that share one must not overlap on the GPU
  * (two captured graphs that may run at once need one each).  sequences <= 4096.
  * With ZTQ_X_F32 or ZTQ_Y_F32 queries (of any size) and weights enter the products with 22 bits, else weights with 11; scores,

@@ -372,3 +372,29 @@ def test_device_error_clears_everything():
     table[0, 1] = -5
     run(lens, cache, table, start, kv_len, q, y, 0.1)
     assert K.device_error() in (6, 7) and K.device_error() == 0
+
+
+# ------------------------------------------------------------------ scales that are not finite, in fp32
+
+@pytest.mark.parametrize("dim,new", [(64, 3), (64, 40), (128, 3), (128, 40), (256, 3)])
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_fp32_scales_that_are_not_finite(dim, new, which, bad):
+    """Blocks in front of the window and unused ones change nothing; the last block makes the rows that see it NaN, and no others."""
+    n, window = 64 + new, 40
+    cache, table, start, kv_len, q, y = attn_case(U.seeded(4), [(n, new)], 2, 4, 16, dim, torch.float32)
+    gone = [b for b in range(cache.blocks) if b not in table[0].tolist()] + table[0, :(n - new - window + 1) // 16].tolist()
+    for t in cache.tensors[2:]:
+        t[gone] = bad
+    run([(n, new)], cache, table, start, kv_len, q, y, 0.1, window)
+    for t in cache.tensors[2:]:
+        t[gone] = 1.0
+    check([(n, new)], cache, table, q, y, 0.1, window, f32=True)
+    cache.tensors[which][int(table[0, (n - 1) // 16]), 1] = bad
+    y.fill_(0.5)
+    run([(n, new)], cache, table, start, kv_len, q, y, 0.1, window)
+    nan = torch.isnan(y[:new])
+    sees = torch.arange(64, n, device=DEV) >= (n - 1) // 16 * 16
+    assert not nan[:, :4].any() and torch.equal(nan[:, 4:].any(-1), sees[:, None].expand(-1, 4))
+    assert which == 2 or torch.equal(nan[:, 4:].all(-1), sees[:, None].expand(-1, 4))
+    no_error()

@@ -138,6 +138,8 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Keys of an infinite scale are infinities of both signs and NaN: so are a row's scores.
+__device__ __forceinline__ float attn_k_scale(float sk) { return fabsf(sk) <= 3.402823466e38f ? sk : __int_as_float(0x7fc00000); }
 // The exponent of a finite V scale
 __device__ __forceinline__ float attn_exponent(float sv) { return (float)max((int)(__float_as_uint(fabsf(sv)) >> 23) - 127, kAttnLeast); }
 // What exponents are moved by for a reference
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(AttnRing<D, NT, SPLIT>::kThreads, 1) attn_rows
             };
             auto scales = [&](int blk) {
                 const long long at = (long long)max(blk, 0) * p.kv_heads + it.h;
-                return blk < 0 ? make_float2(__uint_as_float(kAttnHidden), 0.f) : make_float2(p.ks[at], p.vs[at]);
+                return blk < 0 ? make_float2(__uint_as_float(kAttnHidden), 0.f) : make_float2(attn_k_scale(p.ks[at]), p.vs[at]);
             };
             int blk = look(step0);
             float2 f = scales(blk), f_next = f;

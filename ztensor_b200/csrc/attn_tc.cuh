@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kTcaThreads, 1) attn_tc_kernel(const TcaParams
             const bool fine = fabsf(sc) <= 3.402823466e38f;
             TcaInfo& f = sh.info[i & 3];
             if (warp == 8) {
-                if (lane < 8) f.ks[lane] = fabsf(sc);
+                if (lane < 8) f.ks[lane] = fabsf(attn_k_scale(sc));
                 const uint32_t hidden = __ballot_sync(0xffffffffu, blk < 0) & 255u;
                 if (lane == 0) f.hidden = hidden;
                 __syncwarp();
