@@ -397,7 +397,8 @@ cudaError_t ztq_attn_q8(const void* q, void* y, long long q_token, long long q_h
  * top_k stay (<= 0: all), of those the shortest prefix with top_p of their mass (at least one token; >= 1: all), of those
  * the ones with w >= min_p; the token is the first by index whose running sum of w exceeds uniform times the sum.
  * temperature 0 takes the first of the order.  Per-row arrays; temperature, top_k, top_p, min_p may be NULL (1, all,
- * all, all).  logprob (may be NULL): log of the token's share of what was kept.  -inf and NaN are never drawn; a row
+ * all, all).  w is held in steps of 2^-44 of the largest: a token below 2^-45 counts as 0 and is not drawn, not even for
+ * uniform 0.  logprob (may be NULL): log of the token's share of what was kept.  -inf and NaN are never drawn; a row
  * with nothing else gives token -1 and logprob NaN.  vocab <= ZTQ_SAMPLE_MAX_VOCAB.  Flags: ZTQ_X_F32, ZTQ_NO_PDL. */
 #define ZTQ_SAMPLE_MAX_VOCAB 327680
 cudaError_t ztq_sample(const void* logits, long long row_stride, int rows, int vocab, const float* temperature, const int* top_k,

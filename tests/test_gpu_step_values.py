@@ -398,3 +398,17 @@ def test_fp32_scales_that_are_not_finite(dim, new, which, bad):
     assert not nan[:, :4].any() and torch.equal(nan[:, 4:].any(-1), sees[:, None].expand(-1, 4))
     assert which == 2 or torch.equal(nan[:, 4:].all(-1), sees[:, None].expand(-1, 4))
     no_error()
+
+
+# ------------------------------------------------------------------ sampling
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_tokens_too_light_to_count(f32):
+    """A weight below 2^-45 of the largest is 0 and is not drawn, the smallest above that is: at uniform 0 the first token that has any."""
+    x = torch.full((4, 300), -40.0, dtype=torch.float32 if f32 else torch.float16, device=DEV)
+    x[:, 200] = 0.0
+    x[1, 100], x[2, 100], x[3, 7] = -31.0, -30.0, -60.0      # log2: 44.7, 43.3, 86.6
+    token = torch.zeros(4, dtype=torch.int32, device=DEV)
+    K.sample(x, torch.zeros(4, device=DEV), token)
+    assert token.tolist() == [200, 100, 100, 200]
+    no_error()
