@@ -329,7 +329,7 @@ cudaError_t ztq_kv_plan(const int* ctx_len, const int* new_len, int* block_table
  *   ZTQ_ROPE_BY_TURNS  kept where it makes turns_high turns or more over original_positions, divided by factor where it
  *                      makes turns_low or fewer, a linear blend in the number of turns between
  *   ZTQ_ROPE_BY_DIM    the same, the blend linear in the dimension between those of turns_high (rounded down) and
- *                      turns_low (rounded up)
+ *                      turns_low (rounded up): "NTK-by-parts" (Peng et al., YaRN, 2023)
  * rot_dim: a multiple of 16 up to 256 and the head; what lies behind it in a head passes unchanged. */
 #define ZTQ_ROPE_UNSCALED 0
 #define ZTQ_ROPE_LINEAR   1

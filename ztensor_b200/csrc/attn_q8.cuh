@@ -11,7 +11,7 @@
 // per block, and looks up block table and scales one step ahead; the other warps take 16 tokens of a step in turn.  Twelve of
 // them where 128 registers suffice: a warp's tile is a chain of 380 instructions that eight warps leave half hidden
 // (64 sequences of 3000 to 12000 tokens, 958 MB: 211 us with eight,
-// 192 with twelve and the look-ahead of the producer).
+// 192 with twelve and the look-ahead of the producer, when it was tried).
 //   S^T = K Q^T and Y^T = V^T P^T by mma.sync m16n8k16 with the TOKENS (then the dims) as M and the rows as N = 8: a
 // decode step has 4 to 8 rows per kv head, which as M would waste half of every instruction and more.
 //   The contraction index may be permuted as long as both operands agree, so every lane reads 16 contiguous bytes of the
@@ -31,8 +31,8 @@
 //   A tile of 16 tokens lies in one block (block sizes are multiples of 16), so its scales are two scalars: sk goes into
 // the score's factor, sv into p.
 //
-// Measured: 64 sequences of 3000 to 12000 tokens, 64 / 8 heads of 128 (958 MB) 193 us = 4.96 TB/s, 160 with the arithmetic
-// left out; one sequence of 8192 tokens 18 us with the join, of which the copies and the arithmetic take 4.
+// Measured: 64 sequences of 3000 to 12000 tokens, 64 / 8 heads of 128 (958 MB) 186 to 200 us from box to box (5.15 to 4.8 TB/s),
+// 160 with the arithmetic left out; one sequence of 8192 tokens 18 us with the join, of which the copies and the arithmetic take 4.
 //
 // Work: an item is (sequence, tile of rows, kv head).  The steps of all items in order are dealt to the CTAs in equal
 // contiguous ranges, whatever the lengths, so a long sequence is split and short ones are packed.  A CTA that holds part of
