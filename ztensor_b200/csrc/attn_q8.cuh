@@ -20,14 +20,14 @@
 // pairs two tokens' codes by byte permutes.  P^T is the transposed accumulator of S^T (movmatrix).  tau = 0 5 2 7 4 1 6 3:
 // with the copies' 128-byte swizzle both reads are free of bank conflicts (even and odd g differ in bit 2 of the row, even
 // rows of the c's are all different).  A code becomes fp16 exactly: 0x6400 | (code + 128) is 1152 + code.
-//   Online softmax per warp and row, whose reference c is the largest exponent not of a weight but of a weight TIMES the power of two of
-// its V scale: p = 2^(s - c + 4) sv then stays inside fp16 and ends at 2^-29 of the row's largest such product, whatever the
-// scales of blocks are that the row does not see or hardly weighs.  c moves only when exceeded by more than a slack of 8 (one
-// vote per 16 tokens instead of a reduction); it is not rounded, so that a weight that outweighs all others is exact.  The weights' sum, relative to 2^c too, is up to 2^127 apart from 1, which fp32
-// holds.  Scores, references, sums and accumulators are fp32; p is rounded to
-// fp16 for the second product (relative 2^-11, against fp16 outputs with the same step).  With fp32 inputs or outputs
-// (SPLIT) q and p go in as two fp16 terms each, 22 bits; a row of fp32 queries is first brought near the upper end of fp16's
-// range by a power of two, which its scores are divided by.
+//   Online softmax per warp and row, whose reference c is the largest exponent not of a weight but of a weight TIMES the power
+// of two of its V scale: p = 2^(s - c + 4) sv then stays inside fp16 and ends at 2^-29 of the row's largest such product,
+// whatever the scales of blocks are that the row does not see or hardly weighs.  c moves only when exceeded by more than a
+// slack of 8 (one vote per 16 tokens instead of a reduction); it is not rounded, so that a weight that outweighs all others
+// is exact.  The weights' sum is relative to 2^c too, which may be 2^127 apart from 1: fp32 holds that.
+//   Scores, references, sums and accumulators are fp32; p is rounded to fp16 for the second product (relative 2^-11, against
+// fp16 outputs with the same step).  With fp32 inputs or outputs (SPLIT) q and p go in as two fp16 terms each, 22 bits; a row
+// of fp32 queries is first brought near the upper end of fp16's range by a power of two, which its scores are divided by.
 //   A tile of 16 tokens lies in one block (block sizes are multiples of 16), so its scales are two scalars: sk goes into
 // the score's factor, sv into p.
 //
